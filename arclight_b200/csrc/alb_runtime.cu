@@ -56,10 +56,19 @@ int * device_error_ptr() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lk(mu);
     if (!ptrs[dev]) {
+        // Once per device, never on the hot path.  The first call may come while a
+        // stream is being captured: the relaxed mode lets this thread allocate
+        // then, and the zeroing runs on a stream of its own.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
         int * p = nullptr;
-        if (cudaMalloc(&p, 64) != cudaSuccess) return nullptr;   // once per device, never on the hot path
-        cudaMemset(p, 0, 64);
-        cudaDeviceSynchronize();
+        cudaStream_t s = nullptr;
+        bool ok = cudaMalloc(&p, 64) == cudaSuccess && cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking) == cudaSuccess;
+        ok = ok && cudaMemsetAsync(p, 0, 64, s) == cudaSuccess && cudaStreamSynchronize(s) == cudaSuccess;
+        if (s) cudaStreamDestroy(s);
+        if (!ok && p) cudaFree(p);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (!ok) return nullptr;
         ptrs[dev] = p;
     }
     return ptrs[dev];
