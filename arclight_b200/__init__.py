@@ -20,7 +20,27 @@ ALB_OK = 0
 ALB_ERR_INVALID = -1
 ALB_ERR_NO_SLOT = -7
 ALB_FLASH_ATTN_STATIC_BYTES = 4 << 20   # include/alb_cuda.h
+ALB_KV_F16 = 0
+ALB_KV_BF16 = 1
 _lib = None
+
+
+class PagedKV(C.Structure):
+    """alb_paged_kv (include/alb_cuda.h): a cache of pages and its page table."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("page_stride", C.c_int64), ("cell_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("n_pages", C.c_int64), ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("page_size", C.c_int32),
+                ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("type", C.c_int32)]
+
+
+class LogitsRules(C.Structure):
+    """alb_logits_rules (include/alb_cuda.h): what alb_logits_process applies."""
+    _fields_ = [("history", C.c_void_p), ("history_stride", C.c_int64), ("history_len", C.c_void_p),
+                ("prompt_len", C.c_void_p), ("last_n", C.c_int32), ("repetition", C.c_void_p),
+                ("frequency", C.c_void_p), ("presence", C.c_void_p), ("temperature", C.c_void_p),
+                ("bias_offsets", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p),
+                ("n_bias", C.c_int32), ("allow", C.c_void_p), ("allow_stride", C.c_int64), ("allow_row", C.c_void_p),
+                ("n_allow", C.c_int32)]
 
 
 class AlbError(RuntimeError):
@@ -86,6 +106,10 @@ def _declare(L: C.CDLL) -> None:
         "alb_rope_table": (ci, [vp, i32, i32, f32]),
         "alb_qk_norm_rope_kv": (ci, [vp, i64, i32, i32, vp, vp, f32, vp, i32, vp, vp, vp, vp]),
         "alb_qk_norm_rope_kv_cells": (ci, [vp, i64, i32, i32, vp, vp, f32, vp, i32, vp, vp, i64, vp, vp, vp, vp]),
+        "alb_qk_norm_rope_kv_paged": (ci, [vp, i64, i64, i32, vp, vp, f32, vp, i32, vp, vp, vp, vp, vp]),
+        "alb_paged_attn_workspace_bytes": (sz, [vp, i64, i32]),
+        "alb_paged_attn": (ci, [vp, i64, i32, vp, vp, vp, i32, f32, vp, vp, vp, vp]),
+        "alb_logits_process": (ci, [vp, i64, i64, i64, vp, vp, i64, vp, vp]),
         "alb_flash_attn_workspace_bytes": (sz, [i32, i32, i64, i32, i32]),
         "alb_flash_attn": (ci, [vp, vp, vp, i64, i32, i32, i32, f32, i32, vp, vp, vp]),
         "alb_gemm_workspace_bytes": (C.c_size_t, [i64, i64]),

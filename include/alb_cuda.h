@@ -199,7 +199,121 @@ ALB_API int alb_flash_attn_static(const float * q, const uint16_t * k_cache, con
                                   int32_t n_head, int32_t n_head_kv, int32_t pos0, float scale, int32_t splits,
                                   float * out, void * stream);
 
+/* --------------------------------------------------------- paged K/V cache
+ * A batch of sequences in one cache of fixed-size pages.  The cell of position p
+ * of sequence s is slot p % page_size of page page_table[s][p / page_size]; with
+ * page_size 1 the table holds cell indices, e.g. those of the KV-cache manager
+ * (alb_kv_visible_cells).  No counterpart in the reference, whose cache is one
+ * row of cells per stream with a dense mask (cgraph.cpp:1057-1261). */
+enum {
+    ALB_KV_F16 = 0,
+    ALB_KV_BF16 = 1,
+};
+typedef struct {
+    void *          k;            /* device, fp16 or bf16, 16-byte aligned: element d of head h of slot c of page g is */
+    void *          v;            /*   at g * page_stride + c * cell_stride + h * head_stride + d */
+    const int32_t * page_table;   /* device [n_seqs] rows of max_pages page indices */
+    int64_t         table_stride; /* elements from one row of page_table to the next; 0: max_pages */
+    int64_t         page_stride;  /* elements, multiples of 8; all three 0: dense [n_pages][page_size][n_head_kv][head_dim] */
+    int64_t         cell_stride;
+    int64_t         head_stride;
+    int64_t         n_pages;      /* n_pages * page_size < 2^31 */
+    int32_t         n_seqs;
+    int32_t         max_pages;    /* max_pages * page_size < 2^31 */
+    int32_t         page_size;    /* any size from 1 */
+    int32_t         n_head_kv;
+    int32_t         head_dim;     /* 64 or 128 */
+    int32_t         type;         /* ALB_KV_F16 or ALB_KV_BF16 */
+} alb_paged_kv;
+
+/* alb_qk_norm_rope_kv_cells for a paged cache: token t (row t of qkv, the fused
+ * projection [T][qkv_stride] of (n_head + 2 n_head_kv) * head_dim values;
+ * qkv_stride in elements, a multiple of 4, 0: dense) is position positions[t] of
+ * sequence seqs[t] (device int32; seqs NULL: sequence t).  Its Q and K heads get
+ * RMSNorm * q_norm / k_norm (each may be NULL: that norm is left out) and the
+ * NEOX rotation of rope_table [max_pos][head_dim/2] (cos, sin); K and V go to
+ * their cell, rounded to the cache's type (nearest even), Q to q_out
+ * [T][n_head][head_dim].  A token with a negative position or sequence is
+ * padding: nothing is read or written for it.  A position >= max_pos or beyond
+ * the table's pages, a sequence >= n_seqs or a page outside [0, n_pages) skips
+ * the token and alb_device_error() reports 4.  Two tokens with the same cell
+ * leave one of the two rows there.  qkv, q_norm, k_norm, rope_table and q_out are
+ * 16-byte aligned. */
+ALB_API int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, int64_t T, int32_t n_head,
+                                      const float * q_norm, const float * k_norm, float eps, const float * rope_table,
+                                      int32_t max_pos, const int32_t * positions, const int32_t * seqs,
+                                      const alb_paged_kv * kv, float * q_out, void * stream);
+
+/* Attention of single query tokens over a paged cache: row r (q [n_rows][n_head]
+ * [head_dim]) sees positions [max(0, lengths[r] - window), lengths[r]) of sequence
+ * seqs[r] (device int32; seqs NULL: sequence r; window 0: no limit), its own token
+ * included when that is already in the cache:
+ *   out[r][h] = sum_j exp(s_j - m) V_j / sum_j exp(s_j - m),  s_j = scale q . K_j,
+ * m the largest s_j and h / (n_head / n_head_kv) the K/V head (any whole ratio).
+ * lse [n_rows][n_head] (nullable) gets m + log(sum).  q is not rounded: scores
+ * and sums carry fp32 (24 bits of q and of the probabilities).  The cells' order
+ * of summation follows the lengths of the whole batch; the same call gives the
+ * same bits.  A row that sees nothing (length 0) is 0, its lse -INFINITY; a row
+ * with a negative length is padding and left as it was.  Cells outside a row's
+ * range are not read.  A sequence outside [0, n_seqs) leaves its row without
+ * cells, a length beyond the table is cut to it, and the cells of a page outside
+ * [0, n_pages) are not seen; each makes alb_device_error() report 4.  A prompt's
+ * tokens may be rows too (their own lengths), each reading its cells anew.
+ * Nothing depends on the lengths but the work, so a captured call replays with
+ * new lengths, tables and queries in the same buffers.  workspace:
+ * alb_paged_attn_workspace_bytes() bytes, 16-byte aligned, no state kept in it
+ * between calls; calls that may overlap in time (other streams, two captured
+ * graphs replayed side by side) need one each.  q and out are 16-byte aligned. */
+ALB_API size_t alb_paged_attn_workspace_bytes(const alb_paged_kv * kv, int64_t n_rows, int32_t n_head);
+ALB_API int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, const alb_paged_kv * kv,
+                           const int32_t * seqs, const int32_t * lengths, int32_t window, float scale,
+                           void * workspace, float * out, float * lse, void * stream);
+
 /* -------------------------------------------------------------- sampling */
+/* What alb_logits_process does to a row of logits.  All pointers are device
+ * pointers; one that is NULL leaves its rule out. */
+typedef struct {
+    const int32_t *  history;        /* [rows] rows of token ids, oldest first (prompt and output) */
+    int64_t          history_stride; /* elements between rows, and the most a row holds */
+    const int32_t *  history_len;    /* [rows]: ids in the row; negative: the row is padding, left as it was */
+    const int32_t *  prompt_len;     /* [rows]: the first ids that are prompt (NULL: none) */
+    int32_t          last_n;         /* only the last last_n ids count; 0: all */
+    const float *    repetition;     /* [rows] */
+    const float *    frequency;      /* [rows] */
+    const float *    presence;       /* [rows] */
+    const float *    temperature;    /* [rows] */
+    const int32_t *  bias_offsets;   /* [rows + 1]: row r has entries [bias_offsets[r], bias_offsets[r + 1]) */
+    const int32_t *  bias_ids;       /* [n_bias] */
+    const float *    bias_values;    /* [n_bias] */
+    int32_t          n_bias;
+    const uint32_t * allow;          /* [n_allow] bit masks of n_vocab bits, bit i % 32 of word i / 32: token i allowed */
+    int64_t          allow_stride;   /* words between masks; 0: (n_vocab + 31) / 32 */
+    const int32_t *  allow_row;      /* [rows]: which mask (negative: none); NULL: mask r */
+    int32_t          n_allow;
+} alb_logits_rules;
+
+/* The rules a batch of logits goes through before its tokens are chosen; for
+ * token i of row r, in this order, each step rounded to fp32:
+ *   x += bias                          the last of the row's entries with id i
+ *   x  = x > 0 ? x / rep : x * rep     i among the row's counted history
+ *   x -= frequency * n                 n: how often i is among its counted output
+ *   x -= presence                      if n > 0
+ *   x /= temperature                   if temperature > 0
+ *   x  = -INFINITY                     if the row's mask does not allow i
+ * The counted history are the last last_n ids, the counted output those of them
+ * behind the prompt.  out [rows][out_stride] may be logits itself ([rows]
+ * [stride]; strides in elements, 0: n_vocab), but not overlap it otherwise.
+ * next_token [rows] (nullable) gets the lowest index of the largest value, or -1
+ * when nothing but -INFINITY and NaN is left.  Negative ids in history and
+ * bias_ids are skipped; ids >= n_vocab, lengths beyond history_stride (cut to
+ * it), bias offsets outside [0, n_bias] (cut) and mask rows >= n_allow (no mask)
+ * make alb_device_error() report 4.  Extends sample_none (sampler.cpp:34-36),
+ * the reference's only sampler.  n_vocab <= 2^19 when a history or bias is
+ * given. */
+ALB_API int alb_logits_process(const float * logits, int64_t rows, int64_t n_vocab, int64_t stride,
+                               const alb_logits_rules * rules, float * out, int64_t out_stride, int32_t * next_token,
+                               void * stream);
+
 /* sample_none (sampler.cpp:34-36): first index of the maximum of x[0..n).
  * scratch >= 1024 bytes, zeroed once before first use. */
 ALB_API int alb_argmax(const float * x, int64_t n, void * scratch, int32_t * idx_out, void * stream);
