@@ -122,70 +122,495 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int6
 }
 
 // ---------------------------------------------------------------- attention
-template <bool BF16> __device__ __forceinline__ float from_cache(uint16_t h) {
-    if (BF16) return __uint_as_float((uint32_t)h << 16);
-    return alb_h2f(h);
+// One pass over the cells with the running maximum and sum of a softmax, on the
+// tensor cores (mma m16n8k16, fp32 accumulators), everything in registers.
+//
+// A unit is (row, K/V head, group of up to 8 query heads).  Its cells come in
+// tiles of 16, and all tiles of all units form one line that is cut into equal
+// ranges, one per CTA (k_paged_attn): uneven lengths and few rows load the SMs
+// alike, and nothing depends on the lengths but device code.  In a CTA's
+// segment of a unit warp w takes every fourth tile; the warps join through
+// shared memory, and the pieces of a unit that a range's border cuts are joined
+// by k_paged_attn_join.
+//
+// Score product, S = Q K^T:  A (16 x 16) holds the 8 heads twice, rows 0-7 the
+// leading 11 bits of q and rows 8-15 the rest, so one instruction gives both
+// parts of S and c[0] + c[2], c[1] + c[3] their sum: q keeps 22 bits and more at
+// no extra instruction (bf16 caches: three parts of 8 bits, a second product for
+// the third).  Each row of q is scaled by a power of two first, so that its
+// largest value has 10 bits before the point and no part underflows.
+// Value product, O = P V:  the accumulator layout of S is the A layout of P, so
+// the probabilities never leave their registers; they too are split in rows 0-7
+// and 8-15.  Both products sum over an index whose order is free, so the loads
+// pick it: a lane's 16-byte load of K (8 neighbouring values) feeds two k steps,
+// and of V eight n columns (values 8 g + j of a 64-value half, j = column tile).
+// The value product starts from zero for every tile and is added to the sums
+// in fp32 rounding to nearest: the tensor cores truncate when they accumulate,
+// which a long chain would gather into a bias.
+//
+// Exponents are base 2 and the running maximum is rounded up to a whole number,
+// so rescaling is exact; probabilities are scaled by 2^15 to stay clear of fp16's
+// subnormals (p >= 2^-24 of the largest keeps its leading part normal).
+constexpr int PA_WARPS = 4;
+constexpr int PA_THREADS = 32 * PA_WARPS;
+constexpr int PA_TILE = 16;
+constexpr int PA_CTAS_PER_SM = 3;
+constexpr int PA_MAX_CTAS = 1024;
+constexpr int PA_MIN_TILES = 4;          // a CTA's range is at least a tile per warp
+constexpr float PA_SHIFT = 15.0f;
+
+// What a CTA left unfinished: a piece of the unit its range began inside (head)
+// and of the unit that its range began and did not end (tail).
+struct __align__(16) PaMeta {
+    int32_t head_row, head_unit, head_ends, tail_row, tail_unit, pad[3];
+};
+template <int D> struct PaPiece { float o[8][D]; float m[8], l[8]; };
+
+struct PaArgs {
+    const float * q;
+    PagedView kv;
+    const int32_t * seqs, * lengths;
+    int64_t n_rows;
+    int32_t Hq, G, groups, window;
+    float scale_log2;
+    PaMeta * meta;
+    void * pieces;
+    float * out, * lse;
+    int * err;
+};
+
+// The positions [lo, hi) row r sees; `bad`: its sequence or length was out of range.
+__device__ __forceinline__ void pa_span(const PaArgs & a, int64_t r, int32_t & lo, int32_t & hi, int32_t & seq, bool & bad) {
+    hi = a.lengths[r];
+    seq = a.seqs ? a.seqs[r] : (r < a.kv.n_seqs ? (int32_t)r : -1);
+    lo = 0;
+    bad = false;
+    if (hi <= 0) { hi = 0; return; }
+    const int64_t most = (int64_t)a.kv.max_pages * a.kv.page_size;
+    if ((uint32_t)seq >= (uint32_t)a.kv.n_seqs) { hi = 0; bad = true; }
+    else if (hi > most) { hi = (int32_t)most; bad = true; }
+    if (a.window > 0 && hi > a.window) lo = hi - a.window;
+}
+__device__ __forceinline__ int32_t pa_tiles(const PaArgs & a, int64_t r) {
+    int32_t lo, hi, seq;
+    bool bad;
+    pa_span(a, r, lo, hi, seq, bad);
+    return (int32_t)(((uint32_t)(hi - lo) + PA_TILE - 1) / PA_TILE);
 }
 
-// The plain form: one CTA per (query head, row), its four warps taking every
-// fourth cell, a cell's D products spread over the lanes; online softmax per
-// warp, the warps joined through shared memory.
+__device__ __forceinline__ float pa_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16 bytes from p, or zeros.
+__device__ __forceinline__ uint4 pa_load(const uint16_t * p, bool ok) {
+    uint4 r;
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                 "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+                 "@q ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "r"((uint32_t)ok));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ void pa_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// x and y as packed 16-bit parts of falling weight; each part is the rounding of
+// what the ones before it left (exact differences).
+template <bool BF16>
+__device__ __forceinline__ void pa_split(float x, float y, uint32_t & hi, uint32_t & mid, uint32_t & lo) {
+    if (BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        const float2 hf = __bfloat1622float2(h);
+        const float x1 = x - hf.x, y1 = y - hf.y;
+        const __nv_bfloat162 m = __floats2bfloat162_rn(x1, y1);
+        const float2 mf = __bfloat1622float2(m);
+        const __nv_bfloat162 l = __floats2bfloat162_rn(x1 - mf.x, y1 - mf.y);
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        mid = *reinterpret_cast<const uint32_t *>(&m);
+        lo = *reinterpret_cast<const uint32_t *>(&l);
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 hf = __half22float2(h);
+        const __half2 m = __floats2half2_rn(x - hf.x, y - hf.y);
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        mid = *reinterpret_cast<const uint32_t *>(&m);
+        lo = 0;
+    }
+}
+
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128)
-k_paged_attn(const float * __restrict__ q, int Hq, PagedView kv, const int32_t * __restrict__ seqs,
-             const int32_t * __restrict__ lengths, int32_t window, float scale, float * __restrict__ out,
-             float * __restrict__ lse, int * err) {
-    constexpr int N = D / 32;
-    const int64_t r = blockIdx.x;
-    const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    __shared__ float sm[4], sl[4], so[4][D];
+__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM)
+k_paged_attn(const __grid_constant__ PaArgs a) {
+    constexpr int KL = D / 32, VH = D / 64;       // 16-byte loads of K per cell and lane; 64-value halves of V
+    constexpr int PITCH = D + 4;
+    __shared__ __align__(16) float so[PA_WARPS][8][PITCH];
+    __shared__ float sm[PA_WARPS][8], sl[PA_WARPS][8];
+    __shared__ int64_t warp_sum[PA_WARPS];
+    __shared__ int32_t at_row, at_unit, at_tile;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int cta = blockIdx.x;
     alb_pdl_wait();
-    int32_t len = lengths[r];
-    if (len < 0) { alb_pdl_trigger(); return; }
-    const int32_t seq = seqs ? seqs[r] : (r < kv.n_seqs ? (int32_t)r : -1);
-    const int64_t most = (int64_t)kv.max_pages * kv.page_size;
-    if (seq < 0 || seq >= kv.n_seqs || len > most) {
-        if (threadIdx.x == 0) atomicExch(err, ALB_DEVERR_BAD_INDEX);
-        len = seq < 0 || seq >= kv.n_seqs ? 0 : (int32_t)most;
+    alb_pdl_trigger();   // the join may take its place; it waits for this grid's end
+
+    // ---- the plan: this CTA's range of the line of tiles
+    const int32_t units = a.kv.Hkv * a.groups;
+    const int64_t per_thread = (a.n_rows + PA_THREADS - 1) / PA_THREADS;
+    const int64_t r0 = tid * per_thread, r1 = min(a.n_rows, r0 + per_thread);
+    int64_t mine = 0;
+    for (int64_t r = r0; r < r1; ++r) mine += pa_tiles(a, r);
+    int64_t scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
     }
-    const int32_t first = window > 0 && len > window ? len - window : 0;
-    const int32_t * row = kv.table + (int64_t)(len ? seq : 0) * kv.table_stride;
-    const int64_t head = (int64_t)(h / (Hq / kv.Hkv)) * kv.head_stride + N * lane;
-    float qv[N], o[N], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) { qv[i] = q[(r * Hq + h) * D + N * lane + i]; o[i] = 0.0f; }
-    for (int32_t j = first + warp; j < len; j += 4) {
-        const int64_t cell = cell_offset(kv, row, j);
-        if (cell < 0) {
-            if (lane == 0) atomicExch(err, ALB_DEVERR_BAD_INDEX);
-            continue;
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) s = fmaf(qv[i], from_cache<BF16>(kv.k[cell + head + i]), s);
-        s = alb_warp_sum(s) * scale;
-        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn;
-        const float c = expf(m - base), p = expf(s - base);
-        l = fmaf(l, c, p);
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(o[i], c, p * from_cache<BF16>(kv.v[cell + head + i]));
-        m = mn;
-    }
-    if (lane == 0) { sm[warp] = m; sl[warp] = l; }
-#pragma unroll
-    for (int i = 0; i < N; ++i) so[warp][N * lane + i] = o[i];
+    if (lane == 31) warp_sum[warp] = scan;
     __syncthreads();
-    const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), base = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f, c[4];
+    int64_t before = scan - mine, total = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) { c[w] = expf(sm[w] - base); L = fmaf(sl[w], c[w], L); }
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float a = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) a = fmaf(so[w][d], c[w], a);
-        out[(r * Hq + h) * D + d] = L != 0.0f ? a / L : 0.0f;
+    for (int w = 0; w < PA_WARPS; ++w) {
+        if (w < warp) before += warp_sum[w];
+        total += warp_sum[w];
     }
-    if (lse && threadIdx.x == 0) lse[r * Hq + h] = M + logf(L);
+    before *= units;
+    total *= units;
+    const int64_t want = (total + PA_MIN_TILES - 1) / PA_MIN_TILES;
+    const int64_t ctas = want < gridDim.x ? want : gridDim.x;
+    int64_t start = 0, left = 0;
+    if (cta < ctas) {
+        const int64_t each = total / ctas, more = total - each * ctas;
+        start = cta * each + (cta < more ? cta : more);
+        left = each + (cta < more ? 1 : 0);
+    }
+    if (left > 0 && start >= before && start < before + mine * units) {
+        int64_t rem = start - before;
+        int64_t r = r0;
+        for (;; ++r) {
+            const int64_t here = (int64_t)pa_tiles(a, r) * units;
+            if (rem < here) break;
+            rem -= here;
+        }
+        const int32_t n = pa_tiles(a, r);
+        at_row = (int32_t)r;
+        at_unit = (int32_t)(rem / n);
+        at_tile = (int32_t)(rem % n);
+    }
+    __syncthreads();
+    PaMeta meta = {-1, 0, 0, -1, 0, {0, 0, 0}};
+    int32_t row = at_row, unit = at_unit, tile = at_tile;
+
+    // ---- the segments
+    while (left > 0) {
+        int32_t lo, hi, seq;
+        bool bad;
+        pa_span(a, row, lo, hi, seq, bad);
+        const int32_t all = (int32_t)(((uint32_t)(hi - lo) + PA_TILE - 1) / PA_TILE);
+        const int32_t n = (int32_t)min((int64_t)(all - tile), left);
+        const bool begins = tile == 0, ends = tile + n == all;
+        lo += tile * PA_TILE;
+        const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
+        const int heads = min(8, a.G - 8 * grp);
+        const int32_t head0 = kvh * a.G + 8 * grp;
+        const int32_t * table = a.kv.table + (int64_t)seq * a.kv.table_stride;
+        const uint16_t * kb = a.kv.k + (int64_t)kvh * a.kv.head_stride + 8 * t;
+        const uint16_t * vb = a.kv.v + (int64_t)kvh * a.kv.head_stride + 8 * g;
+
+        // lanes l and l + 16 look after cell l of a tile: its page one tile ahead
+        auto page_at = [&](int32_t i, int32_t & pos) {
+            pos = lo + i * PA_TILE + (lane & 15);
+            if (i >= n || pos >= hi) { pos = -1; return 0; }
+            return __ldg(table + page_of(a.kv, pos));
+        };
+        auto offset_of = [&](int32_t page, int32_t pos) -> int64_t {
+            if (pos < 0) return -1;
+            if ((uint32_t)page >= (uint32_t)a.kv.n_pages) { atomicExch(a.err, ALB_DEVERR_BAD_INDEX); return -1; }
+            const int32_t p = page_of(a.kv, pos);
+            return (int64_t)page * a.kv.page_stride + (int64_t)(pos - p * a.kv.page_size) * a.kv.cell_stride;
+        };
+        int32_t pos, pos2;
+        int32_t page = page_at(warp, pos);
+        int32_t page2 = page_at(warp + PA_WARPS, pos2);
+
+        // q of head g: its values 32 i + 8 t .. + 7 are k steps 2 i and 2 i + 1 of this lane
+        uint32_t qh[KL][4], qm[KL][4], ql[BF16 ? KL : 1][4];
+        float c;
+        {
+            float qv[KL][8];
+            float top = 0.0f;
+            const float * qr = a.q + ((int64_t)row * a.Hq + head0 + g) * D + 8 * t;
+#pragma unroll
+            for (int i = 0; i < KL; ++i) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qv[i][e] = 0.0f;
+                if (g < heads) {
+                    *reinterpret_cast<float4 *>(qv[i]) = *reinterpret_cast<const float4 *>(qr + 32 * i);
+                    *reinterpret_cast<float4 *>(qv[i] + 4) = *reinterpret_cast<const float4 *>(qr + 32 * i + 4);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(qv[i][e]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^e with top 2^e in [2^9, 2^10); nothing to scale for 0 and what is not finite
+            const int ex = (int)(__float_as_uint(top) >> 23);           // biased exponent, 0 for subnormals
+            int e = ex == 255 || top == 0.0f ? 0 : 127 + 9 - max(ex, 1);
+            e = min(e, 126);
+            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+            c = e > 0 ? a.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23)
+                      : a.scale_log2 * (1.0f / up);
+#pragma unroll
+            for (int i = 0; i < KL; ++i)
+#pragma unroll
+                for (int e2 = 0; e2 < 4; ++e2) {
+                    uint32_t h, m, l;
+                    pa_split<BF16>(qv[i][2 * e2] * up, qv[i][2 * e2 + 1] * up, h, m, l);
+                    qh[i][e2] = h;
+                    qm[i][e2] = m;
+                    if (BF16) ql[i][e2] = l;
+                }
+        }
+
+        float o[VH][8][2], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int h = 0; h < VH; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[h][j][0] = o[h][j][1] = 0.0f;
+
+        uint4 K[2][KL], V[4][VH];
+        bool ok[4];
+        auto load_k = [&](int64_t off) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int64_t f = __shfl_sync(0xffffffffu, off, g + 8 * u);
+#pragma unroll
+                for (int i = 0; i < KL; ++i) K[u][i] = pa_load(kb + f + 32 * i, f >= 0);
+            }
+        };
+        auto load_v = [&](int64_t off) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t f = __shfl_sync(0xffffffffu, off, 2 * t + (u & 1) + 4 * (u & 2));
+                ok[u] = f >= 0;
+#pragma unroll
+                for (int h = 0; h < VH; ++h) V[u][h] = pa_load(vb + f + 64 * h, f >= 0);
+            }
+        };
+        int64_t off = offset_of(page, pos);
+        load_k(off);
+        load_v(off);
+        for (int32_t i = warp; i < n; i += PA_WARPS) {
+            float s[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KL; ++k) {
+                    pa_mma<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], K[u][k].x, K[u][k].y);
+                    pa_mma<BF16>(s[u], qh[k][2], qm[k][2], qh[k][3], qm[k][3], K[u][k].z, K[u][k].w);
+                    if (BF16) {
+                        pa_mma<BF16>(s[u], ql[k][0], 0u, ql[k][1], 0u, K[u][k].x, K[u][k].y);
+                        pa_mma<BF16>(s[u], ql[k][2], 0u, ql[k][3], 0u, K[u][k].z, K[u][k].w);
+                    }
+                }
+            }
+            // the next tile's K comes while this tile's softmax and values are worked on
+            off = offset_of(page2, pos2);
+            load_k(off);
+            page2 = page_at(i + 2 * PA_WARPS, pos2);
+
+            float x[4];   // cells 2t, 2t + 1, 2t + 8, 2t + 9
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                x[u] = s[u >> 1][u & 1] + s[u >> 1][2 + (u & 1)];
+                top = fmaxf(top, ok[u] ? __fmul_rn(x[u], c) : -INFINITY);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float mn = fmaxf(m, ceilf(top));
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            const float fix = pa_ex2(m - base);
+            m = mn;
+            // one rounding from the score on, as long as the maximum of the rounded products is
+            // within 2^-8 of the exact ones' (2^16 has steps of 2^-7); the rounded products beyond
+            const bool big = !(fabsf(base) < 65536.0f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                x[u] = !ok[u] ? 0.0f : pa_ex2(big ? __fmul_rn(x[u], c) - base + PA_SHIFT : fmaf(x[u], c, PA_SHIFT - base));
+            l = fmaf(l, fix, (x[0] + x[1]) + (x[2] + x[3]));
+            uint32_t h0, m0, l0, h1, m1, l1;
+            pa_split<BF16>(x[0], x[1], h0, m0, l0);
+            pa_split<BF16>(x[2], x[3], h1, m1, l1);
+#pragma unroll
+            for (int h = 0; h < VH; ++h) {
+                const uint32_t * va = reinterpret_cast<const uint32_t *>(&V[0][h]), * vc = reinterpret_cast<const uint32_t *>(&V[1][h]);
+                const uint32_t * vd = reinterpret_cast<const uint32_t *>(&V[2][h]), * ve = reinterpret_cast<const uint32_t *>(&V[3][h]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+                    const uint32_t b0 = __byte_perm(va[j >> 1], vc[j >> 1], sel);
+                    const uint32_t b1 = __byte_perm(vd[j >> 1], ve[j >> 1], sel);
+                    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (BF16) pa_mma<BF16>(r, l0, 0u, l1, 0u, b0, b1);
+                    pa_mma<BF16>(r, h0, m0, h1, m1, b0, b1);
+                    o[h][j][0] = fmaf(o[h][j][0], fix, r[0] + r[2]);
+                    o[h][j][1] = fmaf(o[h][j][1], fix, r[1] + r[3]);
+                }
+            }
+            load_v(off);
+        }
+
+        // ---- join the warps: thread (head, part) adds its D / 16 values
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t == 0) { sm[warp][g] = m; sl[warp][g] = l; }
+#pragma unroll
+        for (int h = 0; h < VH; ++h)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int j = 0; j < 8; j += 4)
+                    *reinterpret_cast<float4 *>(&so[warp][g][64 * h + 16 * t + 8 * p + j]) =
+                        make_float4(o[h][j][p], o[h][j + 1][p], o[h][j + 2][p], o[h][j + 3][p]);
+        __syncthreads();
+        {
+            constexpr int N = D / 16;
+            const int h = tid >> 4, d = (tid & 15) * N;
+            float M = sm[0][h];
+#pragma unroll
+            for (int w = 1; w < PA_WARPS; ++w) M = fmaxf(M, sm[w][h]);
+            const float base = M == -INFINITY ? 0.0f : M;
+            float Ls = 0.0f, acc[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) {
+                const float f = pa_ex2(sm[w][h] - base);
+                Ls = fmaf(sl[w][h], f, Ls);
+#pragma unroll
+                for (int e = 0; e < N; e += 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(&so[w][h][d + e]);
+                    acc[e] = fmaf(v.x, f, acc[e]);
+                    acc[e + 1] = fmaf(v.y, f, acc[e + 1]);
+                    acc[e + 2] = fmaf(v.z, f, acc[e + 2]);
+                    acc[e + 3] = fmaf(v.w, f, acc[e + 3]);
+                }
+            }
+            if (h < heads) {
+                if (begins && ends) {
+                    float * dst = a.out + ((int64_t)row * a.Hq + head0 + h) * D + d;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) acc[e] = Ls != 0.0f ? acc[e] / Ls : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < N; e += 4)
+                        *reinterpret_cast<float4 *>(dst + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+                    if (a.lse && (tid & 15) == 0)
+                        a.lse[(int64_t)row * a.Hq + head0 + h] =
+                            Ls != 0.0f ? fmaf(M, 0.693147181f, logf(Ls * 0x1p-15f)) : -INFINITY;
+                } else {
+                    PaPiece<D> * piece = static_cast<PaPiece<D> *>(a.pieces) + 2 * cta + (begins ? 1 : 0);
+#pragma unroll
+                    for (int e = 0; e < N; e += 4)
+                        *reinterpret_cast<float4 *>(&piece->o[h][d + e]) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+                    if ((tid & 15) == 0) { piece->m[h] = M; piece->l[h] = Ls; }
+                }
+            }
+            if (!begins) { meta.head_row = row; meta.head_unit = unit; meta.head_ends = ends; }
+            else if (!ends) { meta.tail_row = row; meta.tail_unit = unit; }
+        }
+        __syncthreads();   // the shared sums are free again
+        left -= n;
+        tile = 0;
+        if (left > 0 && ++unit == units) {
+            unit = 0;
+            do ++row; while (pa_tiles(a, row) == 0);
+        }
+    }
+    if (tid == 0) {
+        reinterpret_cast<int4 *>(a.meta + cta)[0] = make_int4(meta.head_row, meta.head_unit, meta.head_ends, meta.tail_row);
+        a.meta[cta].tail_unit = meta.tail_unit;
+    }
+}
+
+// Joins the pieces of the unit that CTA blockIdx.x of k_paged_attn began and did
+// not end (its tail, then the heads of the CTAs behind it up to the one that
+// ends the unit, in that order), writes the rows that see nothing, and reports
+// rows whose sequence or length was out of range.
+template <int D>
+__global__ void __launch_bounds__(256)
+k_paged_attn_join(const __grid_constant__ PaArgs a) {
+    constexpr int PER_HEAD = D / 4;          // threads of a head, four values each
+    constexpr int PARTS = 256 / (8 * PER_HEAD);
+    const int tid = threadIdx.x, cta = blockIdx.x;
+    __shared__ __align__(16) float4 so[PARTS][8][PER_HEAD];
+    __shared__ float sL[PARTS][8];
+    alb_pdl_wait();
+    const PaPiece<D> * pieces = static_cast<const PaPiece<D> *>(a.pieces);
+    const PaMeta * meta = a.meta;
+    if (meta[cta].tail_row >= 0) {           // uniform over the block
+        int last = cta + 1;
+        while (last + 1 < (int)gridDim.x && !meta[last].head_ends) ++last;
+        const int32_t row = meta[cta].tail_row, unit = meta[cta].tail_unit;
+        const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
+        const int heads = min(8, a.G - 8 * grp);
+        const int part = tid / (8 * PER_HEAD), h = tid / PER_HEAD % 8, d = tid % PER_HEAD;
+        auto piece = [&](int i) { return pieces + (i == cta ? 2 * cta + 1 : 2 * i); };
+        float M = -INFINITY;
+        if (h < heads)
+            for (int i = cta; i <= last; ++i) M = fmaxf(M, piece(i)->m[h]);
+        const float base = M == -INFINITY ? 0.0f : M;
+        float Ls = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (h < heads)
+            for (int i = cta + part; i <= last; i += PARTS) {
+                const PaPiece<D> * p = piece(i);
+                const float f = pa_ex2(p->m[h] - base);
+                const float4 v = *reinterpret_cast<const float4 *>(&p->o[h][4 * d]);
+                Ls = fmaf(p->l[h], f, Ls);
+                acc.x = fmaf(v.x, f, acc.x);
+                acc.y = fmaf(v.y, f, acc.y);
+                acc.z = fmaf(v.z, f, acc.z);
+                acc.w = fmaf(v.w, f, acc.w);
+            }
+        so[part][h][d] = acc;
+        if (d == 0) sL[part][h] = Ls;
+        __syncthreads();
+        if (part == 0 && h < heads) {
+#pragma unroll
+            for (int p = 1; p < PARTS; ++p) {
+                const float4 v = so[p][h][d];
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+                Ls += sL[p][h];
+            }
+            const int64_t head = (int64_t)row * a.Hq + kvh * a.G + 8 * grp + h;
+            if (Ls != 0.0f) acc = make_float4(acc.x / Ls, acc.y / Ls, acc.z / Ls, acc.w / Ls);
+            else acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            *reinterpret_cast<float4 *>(a.out + head * D + 4 * d) = acc;
+            if (a.lse && d == 0) a.lse[head] = Ls != 0.0f ? fmaf(M, 0.693147181f, logf(Ls * 0x1p-15f)) : -INFINITY;
+        }
+    }
+    for (int64_t r = cta; r < a.n_rows; r += gridDim.x) {
+        int32_t lo, hi, seq;
+        bool bad;
+        pa_span(a, r, lo, hi, seq, bad);
+        if (bad && tid == 0) atomicExch(a.err, ALB_DEVERR_BAD_INDEX);
+        if (hi > lo || a.lengths[r] < 0) continue;
+        float * o = a.out + r * a.Hq * D;
+        for (int i = tid; i < a.Hq * D / 4; i += 256) reinterpret_cast<float4 *>(o)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (a.lse)
+            for (int i = tid; i < a.Hq; i += 256) a.lse[r * a.Hq + i] = -INFINITY;
+    }
     alb_pdl_trigger();
 }
 
@@ -257,12 +682,16 @@ cudaError_t launch_append(const float * qkv, int64_t qkv_stride, int64_t T, int 
                       qkv_stride, items, Hq, qn, kn, eps, rope, max_pos, positions, seqs, kv, q_out, err);
 }
 
+size_t attn_ws_bytes(int D) {
+    return PA_MAX_CTAS * (sizeof(PaMeta) + 2 * (D == 128 ? sizeof(PaPiece<128>) : sizeof(PaPiece<64>)));
+}
+
 template <int D, bool BF16>
-cudaError_t launch_attn(const float * q, int64_t n_rows, int Hq, const PagedView & kv, const int32_t * seqs,
-                        const int32_t * lengths, int32_t window, float scale, float * out, float * lse, int * err,
-                        cudaStream_t st) {
-    return alb_launch(k_paged_attn<D, BF16>, dim3((unsigned)n_rows, (unsigned)Hq), dim3(128), 0, st, true, q, Hq, kv,
-                      seqs, lengths, window, scale, out, lse, err);
+cudaError_t launch_attn(const PaArgs & a, cudaStream_t st) {
+    const int ctas = min(PA_MAX_CTAS, PA_CTAS_PER_SM * alb_sm_count());
+    cudaError_t e = alb_launch(k_paged_attn<D, BF16>, dim3((unsigned)ctas), dim3(PA_THREADS), 0, st, true, a);
+    if (e != cudaSuccess) return e;
+    return alb_launch(k_paged_attn_join<D>, dim3((unsigned)ctas), dim3(256), 0, st, true, a);
 }
 
 }  // namespace
@@ -290,7 +719,7 @@ extern "C" int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, 
 extern "C" size_t alb_paged_attn_workspace_bytes(const alb_paged_kv * kv, int64_t n_rows, int32_t n_head) {
     PagedView v;
     if (!paged_view(kv, v, false) || n_rows <= 0 || n_head <= 0 || n_head % v.Hkv != 0) return 0;
-    return 16;
+    return attn_ws_bytes(kv->head_dim);
 }
 
 extern "C" int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, const alb_paged_kv * kv,
@@ -299,13 +728,18 @@ extern "C" int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, c
     PagedView v;
     if (!paged_view(kv, v, true)) return ALB_ERR_INVALID;
     ALB_CHECK_ARG(q && lengths && workspace && out && n_rows > 0 && n_rows < ((int64_t)1 << 24) && window >= 0);
-    ALB_CHECK_ARG(n_head > 0 && n_head <= 65535 && n_head % v.Hkv == 0);
+    ALB_CHECK_ARG(n_head > 0 && n_head < 4096 && n_head % v.Hkv == 0);   // 2^24 rows x 2^27 tiles x 2^12 units < 2^63
     ALB_CHECK_ARG(scale > 0.0f && std::isfinite(scale));
     ALB_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0);
-    int * err = device_error_ptr();
-    ALB_CUDA_TRY(err ? cudaSuccess : cudaErrorMemoryAllocation);
+    PaArgs a = {};
+    a.q = q; a.kv = v; a.seqs = seqs; a.lengths = lengths; a.n_rows = n_rows; a.Hq = n_head; a.G = n_head / v.Hkv;
+    a.groups = (a.G + 7) / 8; a.window = window; a.scale_log2 = scale * 1.44269504f; a.out = out; a.lse = lse;
+    a.meta = static_cast<PaMeta *>(workspace);
+    a.pieces = static_cast<uint8_t *>(workspace) + PA_MAX_CTAS * sizeof(PaMeta);
+    a.err = device_error_ptr();
+    ALB_CUDA_TRY(a.err ? cudaSuccess : cudaErrorMemoryAllocation);
     auto * f = kv->head_dim == 128 ? (kv->type == ALB_KV_BF16 ? launch_attn<128, true> : launch_attn<128, false>)
                                    : (kv->type == ALB_KV_BF16 ? launch_attn<64, true> : launch_attn<64, false>);
-    ALB_CUDA_TRY(f(q, n_rows, n_head, v, seqs, lengths, window, scale, out, lse, err, (cudaStream_t)stream));
+    ALB_CUDA_TRY(f(a, (cudaStream_t)stream));
     return ALB_OK;
 }
