@@ -542,46 +542,66 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 
 // Joins the pieces of the unit that CTA blockIdx.x of k_paged_attn began and did
 // not end (its tail, then the heads of the CTAs behind it up to the one that
-// ends the unit, in that order), writes the rows that see nothing, and reports
+// ends the unit), four of its heads per block; the pieces' weights come first,
+// then every thread sums four values of a head over every PARTS-th piece, always
+// in the same order.  The blocks also write the rows that see nothing and report
 // rows whose sequence or length was out of range.
+constexpr int PJ_THREADS = 256, PJ_HEADS = 4;
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(PJ_THREADS)
 k_paged_attn_join(const __grid_constant__ PaArgs a) {
     constexpr int PER_HEAD = D / 4;          // threads of a head, four values each
-    constexpr int PARTS = 256 / (8 * PER_HEAD);
-    const int tid = threadIdx.x, cta = blockIdx.x;
-    __shared__ __align__(16) float4 so[PARTS][8][PER_HEAD];
-    __shared__ float sL[PARTS][8];
+    constexpr int PARTS = PJ_THREADS / (PJ_HEADS * PER_HEAD);
+    const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x, h0 = PJ_HEADS * blockIdx.y;
+    __shared__ __align__(16) float4 so[PARTS][PJ_HEADS][PER_HEAD];
+    __shared__ float sw[PJ_HEADS][PA_MAX_CTAS], sM[PJ_HEADS], sL[PJ_HEADS];
+    __shared__ int s_last;
     alb_pdl_wait();
     const PaPiece<D> * pieces = static_cast<const PaPiece<D> *>(a.pieces);
     const PaMeta * meta = a.meta;
-    if (meta[cta].tail_row >= 0) {           // uniform over the block
-        int last = cta + 1;
-        while (last + 1 < (int)gridDim.x && !meta[last].head_ends) ++last;
-        const int32_t row = meta[cta].tail_row, unit = meta[cta].tail_unit;
-        const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
-        const int heads = min(8, a.G - 8 * grp);
-        const int part = tid / (8 * PER_HEAD), h = tid / PER_HEAD % 8, d = tid % PER_HEAD;
-        auto piece = [&](int i) { return pieces + (i == cta ? 2 * cta + 1 : 2 * i); };
-        float M = -INFINITY;
-        if (h < heads)
-            for (int i = cta; i <= last; ++i) M = fmaxf(M, piece(i)->m[h]);
-        const float base = M == -INFINITY ? 0.0f : M;
-        float Ls = 0.0f;
+    const int32_t row = meta[cta].tail_row, unit = meta[cta].tail_unit;
+    const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
+    const int heads = min(8, a.G - 8 * grp) - h0;
+    if (row >= 0 && heads > 0) {             // uniform over the block
+        if (tid == 0) s_last = gridDim.x - 1;
+        __syncthreads();
+        for (int i = cta + 1 + tid; i < (int)gridDim.x; i += PJ_THREADS)
+            if (meta[i].head_ends) { atomicMin(&s_last, i); break; }
+        __syncthreads();
+        const int n = s_last - cta + 1;      // pieces: this CTA's tail, the heads behind it
+        auto piece = [&](int i) { return pieces + 2 * (cta + i) + (i == 0 ? 1 : 0); };
+        for (int i = tid / PJ_HEADS; i < n; i += PJ_THREADS / PJ_HEADS) sw[tid % PJ_HEADS][i] = piece(i)->m[h0 + tid % PJ_HEADS];
+        __syncthreads();
+        if (tid < 32 * PJ_HEADS) {           // warp h: head h's maximum, weights and sum
+            const int h = tid >> 5;
+            float M = -INFINITY;
+            for (int i = lane; i < n; i += 32) M = fmaxf(M, sw[h][i]);
+            M = alb_warp_max(M);
+            const float base = M == -INFINITY ? 0.0f : M;
+            float l = 0.0f;
+            for (int i = lane; i < n; i += 32) {
+                const float f = pa_ex2(sw[h][i] - base);
+                sw[h][i] = f;
+                l = fmaf(piece(i)->l[h0 + h], f, l);
+            }
+            l = alb_warp_sum(l);
+            if (lane == 0) { sM[h] = M; sL[h] = l; }
+        }
+        __syncthreads();
+        const int part = tid / (PJ_HEADS * PER_HEAD), h = tid / PER_HEAD % PJ_HEADS, d = tid % PER_HEAD;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (h < heads)
-            for (int i = cta + part; i <= last; i += PARTS) {
-                const PaPiece<D> * p = piece(i);
-                const float f = pa_ex2(p->m[h] - base);
-                const float4 v = *reinterpret_cast<const float4 *>(&p->o[h][4 * d]);
-                Ls = fmaf(p->l[h], f, Ls);
+        if (h < heads) {
+#pragma unroll 8
+            for (int i = part; i < n; i += PARTS) {
+                const float f = sw[h][i];
+                const float4 v = *reinterpret_cast<const float4 *>(&piece(i)->o[h0 + h][4 * d]);
                 acc.x = fmaf(v.x, f, acc.x);
                 acc.y = fmaf(v.y, f, acc.y);
                 acc.z = fmaf(v.z, f, acc.z);
                 acc.w = fmaf(v.w, f, acc.w);
             }
+        }
         so[part][h][d] = acc;
-        if (d == 0) sL[part][h] = Ls;
         __syncthreads();
         if (part == 0 && h < heads) {
 #pragma unroll
@@ -591,26 +611,28 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
                 acc.y += v.y;
                 acc.z += v.z;
                 acc.w += v.w;
-                Ls += sL[p][h];
             }
-            const int64_t head = (int64_t)row * a.Hq + kvh * a.G + 8 * grp + h;
-            if (Ls != 0.0f) acc = make_float4(acc.x / Ls, acc.y / Ls, acc.z / Ls, acc.w / Ls);
+            const float L = sL[h];
+            const int64_t head = (int64_t)row * a.Hq + kvh * a.G + 8 * grp + h0 + h;
+            if (L != 0.0f) acc = make_float4(acc.x / L, acc.y / L, acc.z / L, acc.w / L);
             else acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             *reinterpret_cast<float4 *>(a.out + head * D + 4 * d) = acc;
-            if (a.lse && d == 0) a.lse[head] = Ls != 0.0f ? fmaf(M, 0.693147181f, logf(Ls * 0x1p-15f)) : -INFINITY;
+            if (a.lse && d == 0) a.lse[head] = L != 0.0f ? fmaf(sM[h], 0.693147181f, logf(L * 0x1p-15f)) : -INFINITY;
         }
     }
-    for (int64_t r = cta; r < a.n_rows; r += gridDim.x) {
-        int32_t lo, hi, seq;
-        bool bad;
-        pa_span(a, r, lo, hi, seq, bad);
-        if (bad && tid == 0) atomicExch(a.err, ALB_DEVERR_BAD_INDEX);
-        if (hi > lo || a.lengths[r] < 0) continue;
-        float * o = a.out + r * a.Hq * D;
-        for (int i = tid; i < a.Hq * D / 4; i += 256) reinterpret_cast<float4 *>(o)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (a.lse)
-            for (int i = tid; i < a.Hq; i += 256) a.lse[r * a.Hq + i] = -INFINITY;
-    }
+    if (h0 == 0)
+        for (int64_t r = cta; r < a.n_rows; r += gridDim.x) {
+            int32_t lo, hi, seq;
+            bool bad;
+            pa_span(a, r, lo, hi, seq, bad);
+            if (bad && tid == 0) atomicExch(a.err, ALB_DEVERR_BAD_INDEX);
+            if (hi > lo || a.lengths[r] < 0) continue;
+            float * o = a.out + r * a.Hq * D;
+            for (int i = tid; i < a.Hq * D / 4; i += PJ_THREADS)
+                reinterpret_cast<float4 *>(o)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (a.lse)
+                for (int i = tid; i < a.Hq; i += PJ_THREADS) a.lse[r * a.Hq + i] = -INFINITY;
+        }
     alb_pdl_trigger();
 }
 
@@ -691,7 +713,8 @@ cudaError_t launch_attn(const PaArgs & a, cudaStream_t st) {
     const int ctas = min(PA_MAX_CTAS, PA_CTAS_PER_SM * alb_sm_count());
     cudaError_t e = alb_launch(k_paged_attn<D, BF16>, dim3((unsigned)ctas), dim3(PA_THREADS), 0, st, true, a);
     if (e != cudaSuccess) return e;
-    return alb_launch(k_paged_attn_join<D>, dim3((unsigned)ctas), dim3(256), 0, st, true, a);
+    const unsigned parts = (unsigned)(min(a.G, 8) + PJ_HEADS - 1) / PJ_HEADS;
+    return alb_launch(k_paged_attn_join<D>, dim3((unsigned)ctas, parts), dim3(PJ_THREADS), 0, st, true, a);
 }
 
 }  // namespace
