@@ -274,7 +274,7 @@ ALB_API int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, cons
  * pointers; one that is NULL leaves its rule out. */
 typedef struct {
     const int32_t *  history;        /* [rows] rows of token ids, oldest first (prompt and output) */
-    int64_t          history_stride; /* elements between rows, and the most a row holds; < 2^20 */
+    int64_t          history_stride; /* elements between rows, and the most a row holds; < 2^30 */
     const int32_t *  history_len;    /* [rows]: ids in the row; negative: the row is padding, left as it was */
     const int32_t *  prompt_len;     /* [rows]: the first ids that are prompt (NULL: none) */
     int32_t          last_n;         /* only the last last_n ids count; 0: all */
@@ -308,8 +308,7 @@ typedef struct {
  * bias_ids are skipped; ids >= n_vocab, lengths beyond history_stride (cut to
  * it), bias offsets outside [0, n_bias] (cut) and mask rows >= n_allow (no mask)
  * make alb_device_error() report 4.  Extends sample_none (sampler.cpp:34-36),
- * the reference's only sampler.  n_vocab <= 2^30, and <= 2^19 when a history or bias is
- * given. */
+ * the reference's only sampler.  n_vocab <= 450000. */
 ALB_API int alb_logits_process(const float * logits, int64_t rows, int64_t n_vocab, int64_t stride,
                                const alb_logits_rules * rules, float * out, int64_t out_stride, int32_t * next_token,
                                void * stream);
