@@ -33,6 +33,8 @@ template <typename T> struct Entry {
     static constexpr uint32_t PROMPT = 1u << (8 * sizeof(T) - 1), BIASED = PROMPT >> 1, COUNT = BIASED - 1;
 };
 
+constexpr size_t LG_STATIC = 8192;                  // bound of the kernel's static shared memory
+
 struct LogitsArgs {
     const float * x;
     float * y;
@@ -430,7 +432,7 @@ template <typename T, bool TABLE>
 cudaError_t launch_logits(const LogitsArgs & a, int64_t rows, cudaStream_t st) {
     const size_t smem = (size_t)a.granules * LG_GRANULE * (TABLE ? sizeof(T) : 0) + (a.r.allow ? (size_t)a.granules * 16 : 0);
     const unsigned cluster = 1u << a.log_cluster;
-    cudaError_t e = ensure_smem(k_logits<T, TABLE>, smem);
+    cudaError_t e = ensure_smem(k_logits<T, TABLE>, smem + LG_STATIC);   // the limit holds for both kinds together
     if (e == cudaSuccess && cluster > 8)
         e = cudaFuncSetAttribute(k_logits<T, TABLE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;

@@ -147,6 +147,7 @@ def same(x, kw, **more):
     (1, 1, 3, 1, False), (2, 2, 1, 3, True), (3, 31, 50, 4, True), (5, 33, 0, 0, True), (1, 1000, 200, 0, False),
     (7, 1001, 100, 20, True), (4, 32003, 5000, 40, False), (3, 151936, 300, 0, False), (2, 151936, 9000, 300, True),
     (2, 262144, 700, 3, True), (1, 400001, 50, 2, True), (300, 257, 20, 2, True),
+    (9, 185000, 40, 2, True), (9, 96000, 20000, 2, False), (1, 450000, 20000, 2, False),   # shared memory around its limits
 ])
 def test_rules(rows, vocab, hist, bias, mask):
     same(*case(np.random.default_rng(rows * vocab), rows, vocab, hist, bias, mask))
