@@ -22,6 +22,8 @@ struct PagedView {
     int64_t table_stride, page_stride, cell_stride, head_stride;
     int32_t n_pages, n_seqs, max_pages, page_size, Hkv;
     uint32_t div_mul, div_shift;
+    // the attention moves cells' places between lanes as 32-bit numbers of this unit
+    uint32_t page_units, cell_units, unit_bytes;
 };
 
 __device__ __forceinline__ int32_t page_of(const PagedView & kv, int32_t pos) {
@@ -46,79 +48,109 @@ template <> struct Vec<2> { using F = float2; };
 template <> struct Vec<4> { using F = float4; };
 
 // ------------------------------------------------------------------- append
-// One warp per head of a token, N = D/32 neighbouring values per lane, so that
-// the NEOX partner d +- D/2 of every value is the same slot of lane ^ 16.  The
-// arithmetic is k_qk_norm_rope_kv's: fp32 squares summed in double (certified to
-// round to the sequential sum's mean), then the fp32 products in its order.
+// One warp per four heads of a token, N = D/32 neighbouring values of each per
+// lane, so that the NEOX partner d +- D/2 of every value is the same slot of lane
+// ^ 16.  The arithmetic is k_qk_norm_rope_kv's: fp32 squares summed in double
+// (certified to round to the sequential sum's mean), then the fp32 products in
+// its order.  The four sums are folded together (half the lanes keep two of them,
+// a quarter one): 6 exchanges instead of 20, and the eight lanes that end with a
+// head's sum find its scale, all four heads at once.
+constexpr int AP_HEADS = 4, AP_WARPS = 4;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256)
-k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int64_t n_items, int Hq,
-                        const float * __restrict__ qn_w, const float * __restrict__ kn_w, float eps,
-                        const float * __restrict__ rope, int32_t max_pos, const int32_t * __restrict__ positions,
-                        const int32_t * __restrict__ seqs, PagedView kv, float * __restrict__ q_out, int * err) {
+__global__ void __launch_bounds__(32 * AP_WARPS)
+k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int Hq, const float * __restrict__ qn_w,
+                        const float * __restrict__ kn_w, float eps, const float * __restrict__ rope, int32_t max_pos,
+                        const int32_t * __restrict__ positions, const int32_t * __restrict__ seqs, PagedView kv,
+                        float * __restrict__ q_out, int * err) {
     constexpr int N = D / 32;
     using F = typename Vec<N>::F;
     const int lane = threadIdx.x & 31;
-    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t t = blockIdx.x;
+    const int head0 = (blockIdx.y * AP_WARPS + (threadIdx.x >> 5)) * AP_HEADS, H = Hq + 2 * kv.Hkv;
     alb_pdl_wait();
-    if (item >= n_items) { alb_pdl_trigger(); return; }   // (a whole warp; no block barrier follows)
-    const int H = Hq + 2 * kv.Hkv;
-    const int64_t t = item / H;
-    const int head = (int)(item - t * H);
+    alb_pdl_trigger();
+    if (head0 >= H) return;   // (a whole warp; no block barrier follows)
     const int32_t pos = positions[t];
     const int32_t seq = seqs ? seqs[t] : (t < kv.n_seqs ? (int32_t)t : kv.n_seqs);
-    if (pos < 0 || seq < 0) { alb_pdl_trigger(); return; }
+    const float * src = qkv + t * qkv_stride + (int64_t)head0 * D + N * lane;
+    float x[AP_HEADS][N];
+#pragma unroll
+    for (int u = 0; u < AP_HEADS; ++u) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[u][i] = 0.0f;
+        if (head0 + u < H) *reinterpret_cast<F *>(x[u]) = *reinterpret_cast<const F *>(src + u * D);
+    }
+    if (pos < 0 || seq < 0) return;
     const bool in_table = pos < max_pos && seq < kv.n_seqs && page_of(kv, pos) < kv.max_pages;
     const int64_t cell = in_table ? cell_offset(kv, kv.table + (int64_t)seq * kv.table_stride, pos) : -1;
     if (cell < 0) {
         if (lane == 0) atomicExch(err, ALB_DEVERR_BAD_INDEX);
-        alb_pdl_trigger();
         return;
     }
-    const float * src = qkv + t * qkv_stride + (int64_t)head * D;
-    float x[N];
-    *reinterpret_cast<F *>(x) = *reinterpret_cast<const F *>(src + N * lane);
-    if (head < Hq + kv.Hkv) {
-        const float * w = head < Hq ? qn_w : kn_w;
-        if (w) {
-            double s = 0.0;
-#pragma unroll
-            for (int i = 0; i < N; ++i) s += (double)__fmul_rn(x[i], x[i]);
-            s = alb_warp_sum_d(s);
-            if (!alb_rms_mean_certain(s, D)) {   // the reference's sequential sum (the whole warp)
-                s = lane == 0 ? alb_rms_seq_sum(src, D) : 0.0;
-                s = __shfl_sync(0xffffffffu, s, 0);
-            }
-            const float mean = (float)(s / (double)D);
-            const float scale = 1.0f / sqrtf(__fadd_rn(mean, eps));
-            float wv[N];
-            *reinterpret_cast<F *>(wv) = *reinterpret_cast<const F *>(w + N * lane);
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], scale), wv[i]);
-        }
+    if (head0 < Hq + kv.Hkv) {
         float cs[2 * N];
         const float * r = rope + (int64_t)pos * D + 2 * N * (lane & 15);
         *reinterpret_cast<F *>(cs) = *reinterpret_cast<const F *>(r);
         *reinterpret_cast<F *>(cs + N) = *reinterpret_cast<const F *>(r + N);
+        double s[AP_HEADS];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float y = __shfl_xor_sync(0xffffffffu, x[i], 16);
-            x[i] = lane < 16 ? __fsub_rn(__fmul_rn(x[i], cs[2 * i]), __fmul_rn(y, cs[2 * i + 1]))
-                             : __fadd_rn(__fmul_rn(y, cs[2 * i + 1]), __fmul_rn(x[i], cs[2 * i]));
+        for (int u = 0; u < AP_HEADS; ++u) {
+            s[u] = 0.0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[u] += (double)__fmul_rn(x[u][i], x[u][i]);
+        }
+        // lanes with bit 4 keep heads 2 and 3, then lanes with bit 3 the second of their two
+        const bool up = lane & 16, odd = lane & 8;
+        double a = up ? s[2] : s[0], b = up ? s[3] : s[1];
+        a += __shfl_xor_sync(0xffffffffu, up ? s[0] : s[2], 16);
+        b += __shfl_xor_sync(0xffffffffu, up ? s[1] : s[3], 16);
+        double sum = odd ? b : a;
+        sum += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int mine = head0 + (lane >> 3);   // the head whose sum this lane has
+        float mean;
+        if (!alb_rms_mean_cert(sum, D, 1.0 / D, mean) && mine < Hq + kv.Hkv)   // the reference's sequential sum
+            mean = (float)(alb_rms_seq_sum(qkv + t * qkv_stride + (int64_t)mine * D, D) / (double)D);
+        const float scale = 1.0f / sqrtf(__fadd_rn(mean, eps));
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < AP_HEADS; ++u) {
+            const int head = head0 + u;
+            const float sc = __shfl_sync(0xffffffffu, scale, 8 * u);
+            if (head >= Hq + kv.Hkv) continue;
+            const float * w = head < Hq ? qn_w : kn_w;
+            if (w) {
+                float wv[N];
+                *reinterpret_cast<F *>(wv) = *reinterpret_cast<const F *>(w + N * lane);
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[u][i] = __fmul_rn(__fmul_rn(x[u][i], sc), wv[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float y = __shfl_xor_sync(0xffffffffu, x[u][i], 16);
+                x[u][i] = up ? __fadd_rn(__fmul_rn(y, cs[2 * i + 1]), __fmul_rn(x[u][i], cs[2 * i]))
+                             : __fsub_rn(__fmul_rn(x[u][i], cs[2 * i]), __fmul_rn(y, cs[2 * i + 1]));
+            }
         }
     }
-    if (head < Hq) {
-        *reinterpret_cast<F *>(q_out + (t * Hq + head) * D + N * lane) = *reinterpret_cast<F *>(x);
-    } else {
-        const bool is_k = head < Hq + kv.Hkv;
-        const int h = head - Hq - (is_k ? 0 : kv.Hkv);
-        uint16_t * dst = (is_k ? kv.k : kv.v) + cell + (int64_t)h * kv.head_stride + N * lane;
 #pragma unroll
-        for (int i = 0; i < N; i += 2)
-            *reinterpret_cast<uint32_t *>(dst + i) =
-                (uint32_t)to_cache<BF16>(x[i]) | ((uint32_t)to_cache<BF16>(x[i + 1]) << 16);
+    for (int u = 0; u < AP_HEADS; ++u) {
+        const int head = head0 + u;
+        if (head < Hq) {
+            *reinterpret_cast<F *>(q_out + (t * Hq + head) * D + N * lane) = *reinterpret_cast<F *>(x[u]);
+        } else if (head < H) {
+            const bool is_k = head < Hq + kv.Hkv;
+            const int h = head - Hq - (is_k ? 0 : kv.Hkv);
+            uint16_t * dst = (is_k ? kv.k : kv.v) + cell + (int64_t)h * kv.head_stride + N * lane;
+            uint32_t out[N / 2];
+#pragma unroll
+            for (int i = 0; i < N; i += 2)
+                out[i / 2] = (uint32_t)to_cache<BF16>(x[u][i]) | ((uint32_t)to_cache<BF16>(x[u][i + 1]) << 16);
+            if (N == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(out[0], out[N / 2 - 1]);
+            else        *reinterpret_cast<uint32_t *>(dst) = out[0];
+        }
     }
-    alb_pdl_trigger();
 }
 
 // ---------------------------------------------------------------- attention
@@ -203,13 +235,11 @@ __device__ __forceinline__ float pa_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 16 bytes from p, or zeros.
-__device__ __forceinline__ uint4 pa_load(const uint16_t * p, bool ok) {
+__device__ const uint4 pa_zeros[16] = {};   // what a cell that is not seen reads instead
+
+__device__ __forceinline__ uint4 pa_load(const uint16_t * p) {
     uint4 r;
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
-                 "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-                 "@q ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
-                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "r"((uint32_t)ok));
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
 }
 template <bool BF16>
@@ -221,6 +251,17 @@ __device__ __forceinline__ void pa_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from zero.
+template <bool BF16>
+__device__ __forceinline__ void pa_mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // x and y as packed 16-bit parts of falling weight; each part is the rounding of
 // what the ones before it left (exact differences).
@@ -246,7 +287,7 @@ __device__ __forceinline__ void pa_split(float x, float y, uint32_t & hi, uint32
     }
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool FOUR>
 __global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM)
 k_paged_attn(const __grid_constant__ PaArgs a) {
     constexpr int KL = D / 32, VH = D / 64;       // 16-byte loads of K per cell and lane; 64-value halves of V
@@ -319,9 +360,11 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
         const int heads = min(8, a.G - 8 * grp);
         const int32_t head0 = kvh * a.G + 8 * grp;
+        const int gh = FOUR ? g & 3 : g;   // this lane's head
         const int32_t * table = a.kv.table + (int64_t)seq * a.kv.table_stride;
-        const uint16_t * kb = a.kv.k + (int64_t)kvh * a.kv.head_stride + 8 * t;
-        const uint16_t * vb = a.kv.v + (int64_t)kvh * a.kv.head_stride + 8 * g;
+        const uint8_t * kb = reinterpret_cast<const uint8_t *>(a.kv.k + (int64_t)kvh * a.kv.head_stride + 8 * t);
+        const uint8_t * vb = reinterpret_cast<const uint8_t *>(a.kv.v + (int64_t)kvh * a.kv.head_stride + 8 * g);
+        const uint8_t * zeros = reinterpret_cast<const uint8_t *>(pa_zeros);
 
         // lanes l and l + 16 look after cell l of a tile: its page one tile ahead
         auto page_at = [&](int32_t i, int32_t & pos) {
@@ -329,28 +372,27 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             if (i >= n || pos >= hi) { pos = -1; return 0; }
             return __ldg(table + page_of(a.kv, pos));
         };
-        auto offset_of = [&](int32_t page, int32_t pos) -> int64_t {
-            if (pos < 0) return -1;
-            if ((uint32_t)page >= (uint32_t)a.kv.n_pages) { atomicExch(a.err, ALB_DEVERR_BAD_INDEX); return -1; }
-            const int32_t p = page_of(a.kv, pos);
-            return (int64_t)page * a.kv.page_stride + (int64_t)(pos - p * a.kv.page_size) * a.kv.cell_stride;
+        auto offset_of = [&](int32_t page, int32_t pos) -> uint32_t {
+            if (pos < 0) return 0xffffffffu;
+            if ((uint32_t)page >= (uint32_t)a.kv.n_pages) { atomicExch(a.err, ALB_DEVERR_BAD_INDEX); return 0xffffffffu; }
+            return (uint32_t)page * a.kv.page_units + (uint32_t)(pos - page_of(a.kv, pos) * a.kv.page_size) * a.kv.cell_units;
         };
         int32_t pos, pos2;
         int32_t page = page_at(warp, pos);
         int32_t page2 = page_at(warp + PA_WARPS, pos2);
 
         // q of head g: its values 32 i + 8 t .. + 7 are k steps 2 i and 2 i + 1 of this lane
-        uint32_t qh[KL][4], qm[KL][4], ql[BF16 ? KL : 1][4];
+        uint32_t qh[KL][4], qm[KL][4], ql[BF16 && !FOUR ? KL : 1][4];
         float c;
         {
             float qv[KL][8];
             float top = 0.0f;
-            const float * qr = a.q + ((int64_t)row * a.Hq + head0 + g) * D + 8 * t;
+            const float * qr = a.q + ((int64_t)row * a.Hq + head0 + gh) * D + 8 * t;
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) qv[i][e] = 0.0f;
-                if (g < heads) {
+                if (gh < heads) {
                     *reinterpret_cast<float4 *>(qv[i]) = *reinterpret_cast<const float4 *>(qr + 32 * i);
                     *reinterpret_cast<float4 *>(qv[i] + 4) = *reinterpret_cast<const float4 *>(qr + 32 * i + 4);
                 }
@@ -372,9 +414,14 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                 for (int e2 = 0; e2 < 4; ++e2) {
                     uint32_t h, m, l;
                     pa_split<BF16>(qv[i][2 * e2] * up, qv[i][2 * e2 + 1] * up, h, m, l);
-                    qh[i][e2] = h;
-                    qm[i][e2] = m;
-                    if (BF16) ql[i][e2] = l;
+                    if (FOUR) {   // rows 0-3, 4-7, 8-11 of A
+                        qh[i][e2] = g < 4 ? h : m;
+                        qm[i][e2] = g < 4 ? l : 0u;
+                    } else {
+                        qh[i][e2] = h;
+                        qm[i][e2] = m;
+                        if (BF16) ql[i][e2] = l;
+                    }
                 }
         }
 
@@ -386,36 +433,38 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 
         uint4 K[2][KL], V[4][VH];
         bool ok[4];
-        auto load_k = [&](int64_t off) {
+        auto load_k = [&](uint32_t off) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int64_t f = __shfl_sync(0xffffffffu, off, g + 8 * u);
+                const uint32_t f = __shfl_sync(0xffffffffu, off, g + 8 * u);
+                const uint8_t * p = f != 0xffffffffu ? kb + (uint64_t)f * a.kv.unit_bytes : zeros;
 #pragma unroll
-                for (int i = 0; i < KL; ++i) K[u][i] = pa_load(kb + f + 32 * i, f >= 0);
+                for (int i = 0; i < KL; ++i) K[u][i] = pa_load(reinterpret_cast<const uint16_t *>(p) + 32 * i);
             }
         };
-        auto load_v = [&](int64_t off) {
+        auto load_v = [&](uint32_t off) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int64_t f = __shfl_sync(0xffffffffu, off, 2 * t + (u & 1) + 4 * (u & 2));
-                ok[u] = f >= 0;
+                const uint32_t f = __shfl_sync(0xffffffffu, off, 2 * t + (u & 1) + 4 * (u & 2));
+                ok[u] = f != 0xffffffffu;
+                const uint8_t * p = ok[u] ? vb + (uint64_t)f * a.kv.unit_bytes : zeros;
 #pragma unroll
-                for (int h = 0; h < VH; ++h) V[u][h] = pa_load(vb + f + 64 * h, f >= 0);
+                for (int h = 0; h < VH; ++h) V[u][h] = pa_load(reinterpret_cast<const uint16_t *>(p) + 64 * h);
             }
         };
-        int64_t off = offset_of(page, pos);
+        uint32_t off = offset_of(page, pos);
         load_k(off);
         load_v(off);
         for (int32_t i = warp; i < n; i += PA_WARPS) {
             float s[2][4];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < KL; ++k) {
-                    pa_mma<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], K[u][k].x, K[u][k].y);
+                    if (k == 0) pa_mma0<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], K[u][k].x, K[u][k].y);
+                    else        pa_mma<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], K[u][k].x, K[u][k].y);
                     pa_mma<BF16>(s[u], qh[k][2], qm[k][2], qh[k][3], qm[k][3], K[u][k].z, K[u][k].w);
-                    if (BF16) {
+                    if (BF16 && !FOUR) {
                         pa_mma<BF16>(s[u], ql[k][0], 0u, ql[k][1], 0u, K[u][k].x, K[u][k].y);
                         pa_mma<BF16>(s[u], ql[k][2], 0u, ql[k][3], 0u, K[u][k].z, K[u][k].w);
                     }
@@ -431,6 +480,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 x[u] = s[u >> 1][u & 1] + s[u >> 1][2 + (u & 1)];
+                if (FOUR) x[u] += __shfl_xor_sync(0xffffffffu, x[u], 16);   // the parts in rows g and g + 4
                 top = fmaxf(top, ok[u] ? __fmul_rn(x[u], c) : -INFINITY);
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -449,6 +499,12 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             uint32_t h0, m0, l0, h1, m1, l1;
             pa_split<BF16>(x[0], x[1], h0, m0, l0);
             pa_split<BF16>(x[2], x[3], h1, m1, l1);
+            if (FOUR) {
+                h0 = g < 4 ? h0 : m0;
+                h1 = g < 4 ? h1 : m1;
+                m0 = g < 4 ? l0 : 0u;
+                m1 = g < 4 ? l1 : 0u;
+            }
 #pragma unroll
             for (int h = 0; h < VH; ++h) {
                 const uint32_t * va = reinterpret_cast<const uint32_t *>(&V[0][h]), * vc = reinterpret_cast<const uint32_t *>(&V[1][h]);
@@ -458,14 +514,23 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                     const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
                     const uint32_t b0 = __byte_perm(va[j >> 1], vc[j >> 1], sel);
                     const uint32_t b1 = __byte_perm(vd[j >> 1], ve[j >> 1], sel);
-                    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (BF16) pa_mma<BF16>(r, l0, 0u, l1, 0u, b0, b1);
-                    pa_mma<BF16>(r, h0, m0, h1, m1, b0, b1);
+                    float r[4];
+                    pa_mma0<BF16>(r, h0, m0, h1, m1, b0, b1);
+                    if (BF16 && !FOUR) pa_mma<BF16>(r, l0, 0u, l1, 0u, b0, b1);
                     o[h][j][0] = fmaf(o[h][j][0], fix, r[0] + r[2]);
                     o[h][j][1] = fmaf(o[h][j][1], fix, r[1] + r[3]);
                 }
             }
             load_v(off);
+        }
+
+        if (FOUR) {   // the middle parts' products lie with lanes of rows 4-7
+#pragma unroll
+            for (int h = 0; h < VH; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) o[h][j][p] += __shfl_xor_sync(0xffffffffu, o[h][j][p], 16);
         }
 
         // ---- join the warps: thread (head, part) adds its D / 16 values
@@ -541,97 +606,102 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 }
 
 // Joins the pieces of the unit that CTA blockIdx.x of k_paged_attn began and did
-// not end (its tail, then the heads of the CTAs behind it up to the one that
-// ends the unit), four of its heads per block; the pieces' weights come first,
-// then every thread sums four values of a head over every PARTS-th piece, always
-// in the same order.  The blocks also write the rows that see nothing and report
-// rows whose sequence or length was out of range.
-constexpr int PJ_THREADS = 256, PJ_HEADS = 4;
+// not end: its tail, then the heads of the CTAs behind it up to the one that ends
+// the unit.  A block takes two of the unit's heads, a head four warps, a warp
+// every fourth piece and a lane D/32 neighbouring values; the pieces' maxima are
+// whole numbers, so rescaling is exact whatever the order.  The blocks also write
+// the rows that see nothing and report rows whose sequence or length was out of
+// range.
+constexpr int PJ_HEADS = 2, PJ_PARTS = 4, PJ_THREADS = 32 * PJ_HEADS * PJ_PARTS;
 template <int D>
 __global__ void __launch_bounds__(PJ_THREADS)
 k_paged_attn_join(const __grid_constant__ PaArgs a) {
-    constexpr int PER_HEAD = D / 4;          // threads of a head, four values each
-    constexpr int PARTS = PJ_THREADS / (PJ_HEADS * PER_HEAD);
-    const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x, h0 = PJ_HEADS * blockIdx.y;
-    __shared__ __align__(16) float4 so[PARTS][PJ_HEADS][PER_HEAD];
-    __shared__ float sw[PJ_HEADS][PA_MAX_CTAS], sM[PJ_HEADS], sL[PJ_HEADS];
-    __shared__ int s_last;
+    constexpr int N = D / 32;
+    using F = typename Vec<N>::F;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hl = warp / PJ_PARTS, part = warp % PJ_PARTS, cta = blockIdx.x;
+    const int h = PJ_HEADS * blockIdx.y + hl, grid = gridDim.x;
+    __shared__ __align__(16) float so[PJ_HEADS][PJ_PARTS][D];
+    __shared__ float sm[PJ_HEADS][PJ_PARTS], sl[PJ_HEADS][PJ_PARTS];
     alb_pdl_wait();
     const PaPiece<D> * pieces = static_cast<const PaPiece<D> *>(a.pieces);
-    const PaMeta * meta = a.meta;
-    const int32_t row = meta[cta].tail_row, unit = meta[cta].tail_unit;
+    // piece i: the tail of this CTA, then the head of the i-th CTA behind it
+    auto piece = [&](int i) { return pieces + 2 * (cta + i) + (i == 0 ? 1 : 0); };
+    const int32_t row = a.meta[cta].tail_row, unit = a.meta[cta].tail_unit;
     const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
-    const int heads = min(8, a.G - 8 * grp) - h0;
-    if (row >= 0 && heads > 0) {             // uniform over the block
-        if (tid == 0) s_last = gridDim.x - 1;
-        __syncthreads();
-        for (int i = cta + 1 + tid; i < (int)gridDim.x; i += PJ_THREADS)
-            if (meta[i].head_ends) { atomicMin(&s_last, i); break; }
-        __syncthreads();
-        const int n = s_last - cta + 1;      // pieces: this CTA's tail, the heads behind it
-        auto piece = [&](int i) { return pieces + 2 * (cta + i) + (i == 0 ? 1 : 0); };
-        for (int i = tid / PJ_HEADS; i < n; i += PJ_THREADS / PJ_HEADS) sw[tid % PJ_HEADS][i] = piece(i)->m[h0 + tid % PJ_HEADS];
-        __syncthreads();
-        if (tid < 32 * PJ_HEADS) {           // warp h: head h's maximum, weights and sum
-            const int h = tid >> 5;
-            float M = -INFINITY;
-            for (int i = lane; i < n; i += 32) M = fmaxf(M, sw[h][i]);
-            M = alb_warp_max(M);
-            const float base = M == -INFINITY ? 0.0f : M;
-            float l = 0.0f;
-            for (int i = lane; i < n; i += 32) {
-                const float f = pa_ex2(sw[h][i] - base);
-                sw[h][i] = f;
-                l = fmaf(piece(i)->l[h0 + h], f, l);
-            }
-            l = alb_warp_sum(l);
-            if (lane == 0) { sM[h] = M; sL[h] = l; }
-        }
-        __syncthreads();
-        const int part = tid / (PJ_HEADS * PER_HEAD), h = tid / PER_HEAD % PJ_HEADS, d = tid % PER_HEAD;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int heads = min(8, a.G - 8 * grp);
+    if (row >= 0 && PJ_HEADS * (int)blockIdx.y < heads) {   // uniform over the block
+        float M = -INFINITY, L = 0.0f, acc[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = 0.0f;
         if (h < heads) {
-#pragma unroll 8
-            for (int i = part; i < n; i += PARTS) {
-                const float f = sw[h][i];
-                const float4 v = *reinterpret_cast<const float4 *>(&piece(i)->o[h0 + h][4 * d]);
-                acc.x = fmaf(v.x, f, acc.x);
-                acc.y = fmaf(v.y, f, acc.y);
-                acc.z = fmaf(v.z, f, acc.z);
-                acc.w = fmaf(v.w, f, acc.w);
+            bool more = true;
+            for (int i0 = 0; more; i0 += 32) {              // 32 pieces at a time
+                const int i = i0 + lane, c = cta + i;
+                const bool ends = c >= grid || (i > 0 && a.meta[c].head_ends) || c == grid - 1;
+                float m = -INFINITY, l = 0.0f;
+                if (c < grid) { m = piece(i)->m[h]; l = piece(i)->l[h]; }
+                const uint32_t e = __ballot_sync(0xffffffffu, ends);
+                const int n = e ? __ffs(e) : 32;            // pieces of this round
+                more = e == 0u;
+                if (lane >= n || lane % PJ_PARTS != part) { m = -INFINITY; l = 0.0f; }
+                const float Mn = fmaxf(M, alb_warp_max(m)), base = Mn == -INFINITY ? 0.0f : Mn;
+                const float fix = pa_ex2(M - base), f = pa_ex2(m - base);
+                L = fmaf(L, fix, alb_warp_sum(l * f));
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[e] *= fix;
+                M = Mn;
+#pragma unroll
+                for (int u = 0; u < 32 / PJ_PARTS; ++u) {
+                    const int k = PJ_PARTS * u + part;
+                    const float w = __shfl_sync(0xffffffffu, f, k);
+                    if (k < n) {
+                        float v[N];
+                        *reinterpret_cast<F *>(v) = *reinterpret_cast<const F *>(&piece(i0 + k)->o[h][N * lane]);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) acc[e] = fmaf(v[e], w, acc[e]);
+                    }
+                }
             }
         }
-        so[part][h][d] = acc;
+        *reinterpret_cast<F *>(&so[hl][part][N * lane]) = *reinterpret_cast<F *>(acc);
+        if (lane == 0) { sm[hl][part] = M; sl[hl][part] = L; }
         __syncthreads();
         if (part == 0 && h < heads) {
+            float top = sm[hl][0];
 #pragma unroll
-            for (int p = 1; p < PARTS; ++p) {
-                const float4 v = so[p][h][d];
-                acc.x += v.x;
-                acc.y += v.y;
-                acc.z += v.z;
-                acc.w += v.w;
+            for (int p = 1; p < PJ_PARTS; ++p) top = fmaxf(top, sm[hl][p]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            L = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < PJ_PARTS; ++p) {
+                const float f = pa_ex2(sm[hl][p] - base);
+                float v[N];
+                *reinterpret_cast<F *>(v) = *reinterpret_cast<const F *>(&so[hl][p][N * lane]);
+                L = fmaf(sl[hl][p], f, L);
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[e] = fmaf(v[e], f, acc[e]);
             }
-            const float L = sL[h];
-            const int64_t head = (int64_t)row * a.Hq + kvh * a.G + 8 * grp + h0 + h;
-            if (L != 0.0f) acc = make_float4(acc.x / L, acc.y / L, acc.z / L, acc.w / L);
-            else acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            *reinterpret_cast<float4 *>(a.out + head * D + 4 * d) = acc;
-            if (a.lse && d == 0) a.lse[head] = L != 0.0f ? fmaf(sM[h], 0.693147181f, logf(L * 0x1p-15f)) : -INFINITY;
+            const int64_t head = (int64_t)row * a.Hq + kvh * a.G + 8 * grp + h;
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] = L != 0.0f ? acc[e] / L : 0.0f;
+            *reinterpret_cast<F *>(a.out + head * D + N * lane) = *reinterpret_cast<F *>(acc);
+            if (a.lse && lane == 0) a.lse[head] = L != 0.0f ? fmaf(top, 0.693147181f, logf(L * 0x1p-15f)) : -INFINITY;
         }
     }
-    if (h0 == 0)
-        for (int64_t r = cta; r < a.n_rows; r += gridDim.x) {
+    if (blockIdx.y == 0)
+        for (int64_t r = cta; r < a.n_rows; r += grid) {
             int32_t lo, hi, seq;
             bool bad;
             pa_span(a, r, lo, hi, seq, bad);
-            if (bad && tid == 0) atomicExch(a.err, ALB_DEVERR_BAD_INDEX);
+            if (bad && threadIdx.x == 0) atomicExch(a.err, ALB_DEVERR_BAD_INDEX);
             if (hi > lo || a.lengths[r] < 0) continue;
             float * o = a.out + r * a.Hq * D;
-            for (int i = tid; i < a.Hq * D / 4; i += PJ_THREADS)
+            for (int i = threadIdx.x; i < a.Hq * D / 4; i += PJ_THREADS)
                 reinterpret_cast<float4 *>(o)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (a.lse)
-                for (int i = tid; i < a.Hq; i += PJ_THREADS) a.lse[r * a.Hq + i] = -INFINITY;
+                for (int i = threadIdx.x; i < a.Hq; i += PJ_THREADS) a.lse[r * a.Hq + i] = -INFINITY;
         }
     alb_pdl_trigger();
 }
@@ -688,6 +758,15 @@ bool paged_view(const alb_paged_kv * c, PagedView & kv, bool table) {
             span = x.stride * x.count;
         }
     }
+    int64_t unit = 8;
+    while (kv.page_stride % (2 * unit) == 0 && kv.cell_stride % (2 * unit) == 0 && unit < ((int64_t)1 << 30)) unit *= 2;
+    if ((kv.n_pages - 1) * (kv.page_stride / unit) + (kv.page_size - 1) * (kv.cell_stride / unit) >= ((int64_t)1 << 32) - 1) {
+        alb_set_last_error_msg("invalid argument: paged cache strides reach beyond 2^32 units of their common power of two");
+        return false;
+    }
+    kv.page_units = (uint32_t)(kv.page_stride / unit);   // (below 2^32 unless there is one page only, which never steps)
+    kv.cell_units = (uint32_t)(kv.cell_stride / unit);
+    kv.unit_bytes = (uint32_t)(2 * unit);
     uint32_t s = 0;
     while (((uint64_t)1 << s) < (uint64_t)c->page_size) ++s;
     kv.div_shift = s;
@@ -699,9 +778,9 @@ template <int D, bool BF16>
 cudaError_t launch_append(const float * qkv, int64_t qkv_stride, int64_t T, int Hq, const float * qn, const float * kn,
                           float eps, const float * rope, int32_t max_pos, const int32_t * positions,
                           const int32_t * seqs, const PagedView & kv, float * q_out, int * err, cudaStream_t st) {
-    const int64_t items = T * (Hq + 2 * kv.Hkv);
-    return alb_launch(k_qk_norm_rope_kv_paged<D, BF16>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, st, true, qkv,
-                      qkv_stride, items, Hq, qn, kn, eps, rope, max_pos, positions, seqs, kv, q_out, err);
+    const unsigned per_token = (unsigned)(Hq + 2 * kv.Hkv + AP_HEADS * AP_WARPS - 1) / (AP_HEADS * AP_WARPS);
+    return alb_launch(k_qk_norm_rope_kv_paged<D, BF16>, dim3((unsigned)T, per_token), dim3(32 * AP_WARPS), 0, st, true,
+                      qkv, qkv_stride, Hq, qn, kn, eps, rope, max_pos, positions, seqs, kv, q_out, err);
 }
 
 size_t attn_ws_bytes(int D) {
@@ -711,7 +790,8 @@ size_t attn_ws_bytes(int D) {
 template <int D, bool BF16>
 cudaError_t launch_attn(const PaArgs & a, cudaStream_t st) {
     const int ctas = min(PA_MAX_CTAS, PA_CTAS_PER_SM * alb_sm_count());
-    cudaError_t e = alb_launch(k_paged_attn<D, BF16>, dim3((unsigned)ctas), dim3(PA_THREADS), 0, st, true, a);
+    auto * f = BF16 && a.G <= 4 ? k_paged_attn<D, BF16, BF16> : k_paged_attn<D, BF16, false>;
+    cudaError_t e = alb_launch(f, dim3((unsigned)ctas), dim3(PA_THREADS), 0, st, true, a);
     if (e != cudaSuccess) return e;
     const unsigned parts = (unsigned)(min(a.G, 8) + PJ_HEADS - 1) / PJ_HEADS;
     return alb_launch(k_paged_attn_join<D>, dim3((unsigned)ctas, parts), dim3(PJ_THREADS), 0, st, true, a);
@@ -726,7 +806,7 @@ extern "C" int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, 
     PagedView v;
     if (!paged_view(kv, v, true)) return ALB_ERR_INVALID;
     ALB_CHECK_ARG(qkv && rope_table && positions && q_out && T > 0 && max_pos > 0 && eps >= 0.0f);
-    ALB_CHECK_ARG(n_head > 0 && n_head <= 65535 && T <= ((int64_t)1 << 31) / (n_head + 2 * v.Hkv));
+    ALB_CHECK_ARG(n_head > 0 && n_head <= 65535 && T < ((int64_t)1 << 31) / (n_head + 2 * v.Hkv));
     const int64_t dense = (int64_t)(n_head + 2 * v.Hkv) * kv->head_dim;
     ALB_CHECK_ARG(qkv_stride == 0 || (qkv_stride >= dense && qkv_stride % 4 == 0 && qkv_stride < ((int64_t)1 << 31)));
     ALB_CHECK_ARG((((uintptr_t)qkv | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)rope_table | (uintptr_t)q_out) & 15) == 0);

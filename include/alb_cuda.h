@@ -214,7 +214,9 @@ typedef struct {
     void *          v;            /*   at g * page_stride + c * cell_stride + h * head_stride + d */
     const int32_t * page_table;   /* device [n_seqs] rows of max_pages page indices */
     int64_t         table_stride; /* elements from one row of page_table to the next; 0: max_pages */
-    int64_t         page_stride;  /* elements, multiples of 8; all three 0: dense [n_pages][page_size][n_head_kv][head_dim] */
+    int64_t         page_stride;  /* elements, multiples of 8; all three 0: dense [n_pages][page_size][n_head_kv][head_dim];
+                                   * in units of the largest power of two that divides page and cell stride, cells
+                                   * lie within 2^32 - 1 (2^35 elements at the least) */
     int64_t         cell_stride;
     int64_t         head_stride;
     int64_t         n_pages;      /* n_pages * page_size < 2^31 */
@@ -234,7 +236,7 @@ typedef struct {
  * NEOX rotation of rope_table [max_pos][head_dim/2] (cos, sin); K and V go to
  * their cell, rounded to the cache's type (nearest even), Q to q_out
  * [T][n_head][head_dim].  A token with a negative position or sequence is
- * padding: nothing is read or written for it.  A position >= max_pos or beyond
+ * padding: nothing is written for it.  A position >= max_pos or beyond
  * the table's pages, a sequence >= n_seqs or a page outside [0, n_pages) skips
  * the token and alb_device_error() reports 4.  Two tokens with the same cell
  * leave one of the two rows there.  qkv, q_norm, k_norm, rope_table and q_out are
