@@ -186,15 +186,17 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = 32 * PA_WARPS;
 constexpr int PA_TILE = 16;
-constexpr int PA_CTAS_PER_SM = 3;
+// CTAs per SM: what the registers allow (168 a thread at D = 128, 128 at D = 64)
+template <int D> constexpr int PA_CTAS_PER_SM = D == 128 ? 3 : 4;
 constexpr int PA_MAX_CTAS = 1024;
 constexpr int PA_MIN_TILES = 4;          // a CTA's range is at least a tile per warp
 constexpr float PA_SHIFT = 15.0f;
 
-// What a CTA left unfinished: a piece of the unit its range began inside (head)
-// and of the unit that its range began and did not end (tail).
-struct __align__(16) PaMeta {
-    int32_t head_row, head_unit, head_ends, tail_row, tail_unit, pad[3];
+// What each CTA left unfinished: the unit that its range began and did not end
+// (its tail; row -1: none), and whether the unit that its range began inside of
+// (its head) ends there.
+struct PaMeta {
+    int32_t tail_row[PA_MAX_CTAS], tail_unit[PA_MAX_CTAS], head_ends[PA_MAX_CTAS];
 };
 template <int D> struct PaPiece { float o[8][D]; float m[8], l[8]; };
 
@@ -288,7 +290,7 @@ __device__ __forceinline__ void pa_split(float x, float y, uint32_t & hi, uint32
 }
 
 template <int D, bool BF16, bool FOUR>
-__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM)
+__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM<D>)
 k_paged_attn(const __grid_constant__ PaArgs a) {
     constexpr int KL = D / 32, VH = D / 64;       // 16-byte loads of K per cell and lane; 64-value halves of V
     constexpr int PITCH = D + 4;
@@ -345,8 +347,21 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         at_tile = (int32_t)(rem % n);
     }
     __syncthreads();
-    PaMeta meta = {-1, 0, 0, -1, 0, {0, 0, 0}};
+    int32_t tail_row = -1, tail_unit = 0, head_ends = 0;
     int32_t row = at_row, unit = at_unit, tile = at_tile;
+
+    // ---- rows that see nothing, dealt out over the CTAs; rows out of range are reported
+    for (int64_t r = cta; r < a.n_rows; r += gridDim.x) {
+        int32_t lo, hi, seq;
+        bool bad;
+        pa_span(a, r, lo, hi, seq, bad);
+        if (bad && tid == 0) atomicExch(a.err, ALB_DEVERR_BAD_INDEX);
+        if (hi > lo || a.lengths[r] < 0) continue;
+        float * o = a.out + r * a.Hq * D;
+        for (int i = tid; i < a.Hq * D / 4; i += PA_THREADS) reinterpret_cast<float4 *>(o)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (a.lse)
+            for (int i = tid; i < a.Hq; i += PA_THREADS) a.lse[r * a.Hq + i] = -INFINITY;
+    }
 
     // ---- the segments
     while (left > 0) {
@@ -382,11 +397,9 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         int32_t page2 = page_at(warp + PA_WARPS, pos2);
 
         // q of head g: its values 32 i + 8 t .. + 7 are k steps 2 i and 2 i + 1 of this lane
-        uint32_t qh[KL][4], qm[KL][4], ql[BF16 && !FOUR ? KL : 1][4];
-        float c;
+        float qv[KL][8];
+        float top = 0.0f;
         {
-            float qv[KL][8];
-            float top = 0.0f;
             const float * qr = a.q + ((int64_t)row * a.Hq + head0 + gh) * D + 8 * t;
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
@@ -396,9 +409,39 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                     *reinterpret_cast<float4 *>(qv[i]) = *reinterpret_cast<const float4 *>(qr + 32 * i);
                     *reinterpret_cast<float4 *>(qv[i] + 4) = *reinterpret_cast<const float4 *>(qr + 32 * i + 4);
                 }
+            }
+        }
+        uint4 K[2][KL], V[4][VH];
+        bool ok[4];
+        auto load_k = [&](uint32_t off) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t f = __shfl_sync(0xffffffffu, off, g + 8 * u);
+                const uint8_t * p = f != 0xffffffffu ? kb + (uint64_t)f * a.kv.unit_bytes : zeros;
+#pragma unroll
+                for (int i = 0; i < KL; ++i) K[u][i] = pa_load(reinterpret_cast<const uint16_t *>(p) + 32 * i);
+            }
+        };
+        auto load_v = [&](uint32_t off) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t f = __shfl_sync(0xffffffffu, off, 2 * t + (u & 1) + 4 * (u & 2));
+                ok[u] = f != 0xffffffffu;
+                const uint8_t * p = ok[u] ? vb + (uint64_t)f * a.kv.unit_bytes : zeros;
+#pragma unroll
+                for (int h = 0; h < VH; ++h) V[u][h] = pa_load(reinterpret_cast<const uint16_t *>(p) + 64 * h);
+            }
+        };
+        uint32_t off = offset_of(page, pos);
+        load_k(off);
+        load_v(off);
+        uint32_t qh[KL][4], qm[KL][4], ql[BF16 && !FOUR ? KL : 1][4];
+        float c;
+        {
+#pragma unroll
+            for (int i = 0; i < KL; ++i)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(qv[i][e]));
-            }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // 2^e with top 2^e in [2^9, 2^10); nothing to scale for 0 and what is not finite
@@ -431,30 +474,6 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[h][j][0] = o[h][j][1] = 0.0f;
 
-        uint4 K[2][KL], V[4][VH];
-        bool ok[4];
-        auto load_k = [&](uint32_t off) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t f = __shfl_sync(0xffffffffu, off, g + 8 * u);
-                const uint8_t * p = f != 0xffffffffu ? kb + (uint64_t)f * a.kv.unit_bytes : zeros;
-#pragma unroll
-                for (int i = 0; i < KL; ++i) K[u][i] = pa_load(reinterpret_cast<const uint16_t *>(p) + 32 * i);
-            }
-        };
-        auto load_v = [&](uint32_t off) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint32_t f = __shfl_sync(0xffffffffu, off, 2 * t + (u & 1) + 4 * (u & 2));
-                ok[u] = f != 0xffffffffu;
-                const uint8_t * p = ok[u] ? vb + (uint64_t)f * a.kv.unit_bytes : zeros;
-#pragma unroll
-                for (int h = 0; h < VH; ++h) V[u][h] = pa_load(reinterpret_cast<const uint16_t *>(p) + 64 * h);
-            }
-        };
-        uint32_t off = offset_of(page, pos);
-        load_k(off);
-        load_v(off);
         for (int32_t i = warp; i < n; i += PA_WARPS) {
             float s[2][4];
 #pragma unroll
@@ -588,8 +607,8 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                     if ((tid & 15) == 0) { piece->m[h] = M; piece->l[h] = Ls; }
                 }
             }
-            if (!begins) { meta.head_row = row; meta.head_unit = unit; meta.head_ends = ends; }
-            else if (!ends) { meta.tail_row = row; meta.tail_unit = unit; }
+            if (!begins) head_ends = ends;
+            else if (!ends) { tail_row = row; tail_unit = unit; }
         }
         __syncthreads();   // the shared sums are free again
         left -= n;
@@ -600,18 +619,19 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         }
     }
     if (tid == 0) {
-        reinterpret_cast<int4 *>(a.meta + cta)[0] = make_int4(meta.head_row, meta.head_unit, meta.head_ends, meta.tail_row);
-        a.meta[cta].tail_unit = meta.tail_unit;
+        a.meta->tail_row[cta] = tail_row;
+        a.meta->tail_unit[cta] = tail_unit;
+        a.meta->head_ends[cta] = head_ends;
     }
 }
 
 // Joins the pieces of the unit that CTA blockIdx.x of k_paged_attn began and did
 // not end: its tail, then the heads of the CTAs behind it up to the one that ends
 // the unit.  A block takes two of the unit's heads, a head four warps, a warp
-// every fourth piece and a lane D/32 neighbouring values; the pieces' maxima are
-// whole numbers, so rescaling is exact whatever the order.  The blocks also write
-// the rows that see nothing and report rows whose sequence or length was out of
-// range.
+// every fourth piece and a lane D/32 neighbouring values.  What tells whether
+// there is work, where it ends and what the pieces weigh is loaded at once, 128
+// pieces a round; the pieces' maxima are whole numbers, so rescaling is exact
+// whatever the order.
 constexpr int PJ_HEADS = 2, PJ_PARTS = 4, PJ_THREADS = 32 * PJ_HEADS * PJ_PARTS;
 template <int D>
 __global__ void __launch_bounds__(PJ_THREADS)
@@ -626,41 +646,54 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
     const PaPiece<D> * pieces = static_cast<const PaPiece<D> *>(a.pieces);
     // piece i: the tail of this CTA, then the head of the i-th CTA behind it
     auto piece = [&](int i) { return pieces + 2 * (cta + i) + (i == 0 ? 1 : 0); };
-    const int32_t row = a.meta[cta].tail_row, unit = a.meta[cta].tail_unit;
+    // lane l looks after pieces 4 l .. 4 l + 3 of a round for where the unit ends, after 4 l + part for its weight
+    static_assert(PJ_PARTS == 4, "four pieces per lane");
+    int last;                 // place of the first end among this lane's four, or 4
+    float m, l;
+    auto look = [&](int i0) {
+        int ends[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = cta + i0 + 4 * lane + u;
+            ends[u] = c >= grid - 1 ? 1 : i0 + lane + u > 0 ? a.meta->head_ends[c] : 0;
+        }
+        const int i = i0 + 4 * lane + part;
+        m = -INFINITY;
+        l = 0.0f;
+        if (cta + i < grid) { m = piece(i)->m[h]; l = piece(i)->l[h]; }
+        last = ends[0] ? 0 : ends[1] ? 1 : ends[2] ? 2 : ends[3] ? 3 : 4;
+    };
+    const int32_t row = a.meta->tail_row[cta], unit = a.meta->tail_unit[cta];
     const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
     const int heads = min(8, a.G - 8 * grp);
     if (row >= 0 && PJ_HEADS * (int)blockIdx.y < heads) {   // uniform over the block
+        look(0);
         float M = -INFINITY, L = 0.0f, acc[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] = 0.0f;
         if (h < heads) {
-            bool more = true;
-            for (int i0 = 0; more; i0 += 32) {              // 32 pieces at a time
-                const int i = i0 + lane, c = cta + i;
-                const bool ends = c >= grid || (i > 0 && a.meta[c].head_ends) || c == grid - 1;
-                float m = -INFINITY, l = 0.0f;
-                if (c < grid) { m = piece(i)->m[h]; l = piece(i)->l[h]; }
-                const uint32_t e = __ballot_sync(0xffffffffu, ends);
-                const int n = e ? __ffs(e) : 32;            // pieces of this round
-                more = e == 0u;
-                if (lane >= n || lane % PJ_PARTS != part) { m = -INFINITY; l = 0.0f; }
+            for (int i0 = 0;;) {
+                const uint32_t e = __ballot_sync(0xffffffffu, last < 4);
+                const int who = e ? __ffs(e) - 1 : 31;
+                const int n = e ? 4 * who + __shfl_sync(0xffffffffu, last, who) + 1 : 128;   // pieces of this round
+                if (4 * lane + part >= n) { m = -INFINITY; l = 0.0f; }
                 const float Mn = fmaxf(M, alb_warp_max(m)), base = Mn == -INFINITY ? 0.0f : Mn;
                 const float fix = pa_ex2(M - base), f = pa_ex2(m - base);
                 L = fmaf(L, fix, alb_warp_sum(l * f));
 #pragma unroll
-                for (int e = 0; e < N; ++e) acc[e] *= fix;
+                for (int k = 0; k < N; ++k) acc[k] *= fix;
                 M = Mn;
-#pragma unroll
-                for (int u = 0; u < 32 / PJ_PARTS; ++u) {
-                    const int k = PJ_PARTS * u + part;
+#pragma unroll 8
+                for (int k = 0; 4 * k + part < n; ++k) {
                     const float w = __shfl_sync(0xffffffffu, f, k);
-                    if (k < n) {
-                        float v[N];
-                        *reinterpret_cast<F *>(v) = *reinterpret_cast<const F *>(&piece(i0 + k)->o[h][N * lane]);
+                    float v[N];
+                    *reinterpret_cast<F *>(v) = *reinterpret_cast<const F *>(&piece(i0 + 4 * k + part)->o[h][N * lane]);
 #pragma unroll
-                        for (int e = 0; e < N; ++e) acc[e] = fmaf(v[e], w, acc[e]);
-                    }
+                    for (int j = 0; j < N; ++j) acc[j] = fmaf(v[j], w, acc[j]);
                 }
+                if (e) break;
+                i0 += 128;
+                look(i0);
             }
         }
         *reinterpret_cast<F *>(&so[hl][part][N * lane]) = *reinterpret_cast<F *>(acc);
@@ -690,19 +723,6 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
             if (a.lse && lane == 0) a.lse[head] = L != 0.0f ? fmaf(top, 0.693147181f, logf(L * 0x1p-15f)) : -INFINITY;
         }
     }
-    if (blockIdx.y == 0)
-        for (int64_t r = cta; r < a.n_rows; r += grid) {
-            int32_t lo, hi, seq;
-            bool bad;
-            pa_span(a, r, lo, hi, seq, bad);
-            if (bad && threadIdx.x == 0) atomicExch(a.err, ALB_DEVERR_BAD_INDEX);
-            if (hi > lo || a.lengths[r] < 0) continue;
-            float * o = a.out + r * a.Hq * D;
-            for (int i = threadIdx.x; i < a.Hq * D / 4; i += PJ_THREADS)
-                reinterpret_cast<float4 *>(o)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (a.lse)
-                for (int i = threadIdx.x; i < a.Hq; i += PJ_THREADS) a.lse[r * a.Hq + i] = -INFINITY;
-        }
     alb_pdl_trigger();
 }
 
@@ -784,12 +804,12 @@ cudaError_t launch_append(const float * qkv, int64_t qkv_stride, int64_t T, int 
 }
 
 size_t attn_ws_bytes(int D) {
-    return PA_MAX_CTAS * (sizeof(PaMeta) + 2 * (D == 128 ? sizeof(PaPiece<128>) : sizeof(PaPiece<64>)));
+    return sizeof(PaMeta) + 2 * PA_MAX_CTAS * (D == 128 ? sizeof(PaPiece<128>) : sizeof(PaPiece<64>));
 }
 
 template <int D, bool BF16>
 cudaError_t launch_attn(const PaArgs & a, cudaStream_t st) {
-    const int ctas = min(PA_MAX_CTAS, PA_CTAS_PER_SM * alb_sm_count());
+    const int ctas = min(PA_MAX_CTAS, PA_CTAS_PER_SM<D> * alb_sm_count());
     auto * f = BF16 && a.G <= 4 ? k_paged_attn<D, BF16, BF16> : k_paged_attn<D, BF16, false>;
     cudaError_t e = alb_launch(f, dim3((unsigned)ctas), dim3(PA_THREADS), 0, st, true, a);
     if (e != cudaSuccess) return e;
@@ -838,7 +858,7 @@ extern "C" int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, c
     a.q = q; a.kv = v; a.seqs = seqs; a.lengths = lengths; a.n_rows = n_rows; a.Hq = n_head; a.G = n_head / v.Hkv;
     a.groups = (a.G + 7) / 8; a.window = window; a.scale_log2 = scale * 1.44269504f; a.out = out; a.lse = lse;
     a.meta = static_cast<PaMeta *>(workspace);
-    a.pieces = static_cast<uint8_t *>(workspace) + PA_MAX_CTAS * sizeof(PaMeta);
+    a.pieces = static_cast<uint8_t *>(workspace) + sizeof(PaMeta);
     a.err = device_error_ptr();
     ALB_CUDA_TRY(a.err ? cudaSuccess : cudaErrorMemoryAllocation);
     auto * f = kv->head_dim == 128 ? (kv->type == ALB_KV_BF16 ? launch_attn<128, true> : launch_attn<128, false>)
