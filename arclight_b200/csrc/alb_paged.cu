@@ -158,7 +158,7 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // tensor cores (mma m16n8k16, fp32 accumulators), everything in registers.
 //
 // A unit is (row, K/V head, group of up to 8 query heads).  Its cells come in
-// tiles of 16, and all tiles of all units form one line that is cut into equal
+// tiles of 16 (D = 128) or 32, and all tiles of all units form one line that is cut into equal
 // ranges, one per CTA (k_paged_attn): uneven lengths and few rows load the SMs
 // alike, and nothing depends on the lengths but device code.  In a CTA's
 // segment of a unit warp w takes every fourth tile; the warps join through
@@ -185,9 +185,9 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // subnormals (p >= 2^-24 of the largest keeps its leading part normal).
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = 32 * PA_WARPS;
-constexpr int PA_TILE = 16;
-// CTAs per SM: what the registers allow (168 a thread at D = 128, 128 at D = 64)
-template <int D> constexpr int PA_CTAS_PER_SM = D == 128 ? 3 : 4;
+constexpr int PA_CTAS_PER_SM = 3;        // what the registers allow (168 a thread)
+// Cells of a tile: 16 per product step, 8 KB of K and V in a warp's registers either way.
+template <int D> constexpr int PA_TILE = 16 * 128 / D;
 constexpr int PA_MAX_CTAS = 1024;
 constexpr int PA_MIN_TILES = 4;          // a CTA's range is at least a tile per warp
 constexpr float PA_SHIFT = 15.0f;
@@ -195,10 +195,12 @@ constexpr float PA_SHIFT = 15.0f;
 // What each CTA left unfinished: the unit that its range began and did not end
 // (its tail; row -1: none), and whether the unit that its range began inside of
 // (its head) ends there.
+// The pieces' maxima and sums by head, [0] the CTA's head, [1] its tail.
 struct PaMeta {
     int32_t tail_row[PA_MAX_CTAS], tail_unit[PA_MAX_CTAS], head_ends[PA_MAX_CTAS];
+    float m[2][8][PA_MAX_CTAS], l[2][8][PA_MAX_CTAS];
 };
-template <int D> struct PaPiece { float o[8][D]; float m[8], l[8]; };
+template <int D> struct PaPiece { float o[8][D]; };
 
 struct PaArgs {
     const float * q;
@@ -225,11 +227,11 @@ __device__ __forceinline__ void pa_span(const PaArgs & a, int64_t r, int32_t & l
     else if (hi > most) { hi = (int32_t)most; bad = true; }
     if (a.window > 0 && hi > a.window) lo = hi - a.window;
 }
-__device__ __forceinline__ int32_t pa_tiles(const PaArgs & a, int64_t r) {
+template <int TILE> __device__ __forceinline__ int32_t pa_tiles(const PaArgs & a, int64_t r) {
     int32_t lo, hi, seq;
     bool bad;
     pa_span(a, r, lo, hi, seq, bad);
-    return (int32_t)(((uint32_t)(hi - lo) + PA_TILE - 1) / PA_TILE);
+    return (int32_t)(((uint32_t)(hi - lo) + TILE - 1) / TILE);
 }
 
 __device__ __forceinline__ float pa_ex2(float x) {
@@ -290,9 +292,10 @@ __device__ __forceinline__ void pa_split(float x, float y, uint32_t & hi, uint32
 }
 
 template <int D, bool BF16, bool FOUR>
-__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM<D>)
+__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM)
 k_paged_attn(const __grid_constant__ PaArgs a) {
     constexpr int KL = D / 32, VH = D / 64;       // 16-byte loads of K per cell and lane; 64-value halves of V
+    constexpr int TILE = PA_TILE<D>, SUB = TILE / 16;
     constexpr int PITCH = D + 4;
     __shared__ __align__(16) float so[PA_WARPS][8][PITCH];
     __shared__ float sm[PA_WARPS][8], sl[PA_WARPS][8];
@@ -308,7 +311,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
     const int64_t per_thread = (a.n_rows + PA_THREADS - 1) / PA_THREADS;
     const int64_t r0 = tid * per_thread, r1 = min(a.n_rows, r0 + per_thread);
     int64_t mine = 0;
-    for (int64_t r = r0; r < r1; ++r) mine += pa_tiles(a, r);
+    for (int64_t r = r0; r < r1; ++r) mine += pa_tiles<TILE>(a, r);
     int64_t scan = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -337,11 +340,11 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         int64_t rem = start - before;
         int64_t r = r0;
         for (;; ++r) {
-            const int64_t here = (int64_t)pa_tiles(a, r) * units;
+            const int64_t here = (int64_t)pa_tiles<TILE>(a, r) * units;
             if (rem < here) break;
             rem -= here;
         }
-        const int32_t n = pa_tiles(a, r);
+        const int32_t n = pa_tiles<TILE>(a, r);
         at_row = (int32_t)r;
         at_unit = (int32_t)(rem / n);
         at_tile = (int32_t)(rem % n);
@@ -368,10 +371,10 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         int32_t lo, hi, seq;
         bool bad;
         pa_span(a, row, lo, hi, seq, bad);
-        const int32_t all = (int32_t)(((uint32_t)(hi - lo) + PA_TILE - 1) / PA_TILE);
+        const int32_t all = (int32_t)(((uint32_t)(hi - lo) + TILE - 1) / TILE);
         const int32_t n = (int32_t)min((int64_t)(all - tile), left);
         const bool begins = tile == 0, ends = tile + n == all;
-        lo += tile * PA_TILE;
+        lo += tile * TILE;
         const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
         const int heads = min(8, a.G - 8 * grp);
         const int32_t head0 = kvh * a.G + 8 * grp;
@@ -381,9 +384,9 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         const uint8_t * vb = reinterpret_cast<const uint8_t *>(a.kv.v + (int64_t)kvh * a.kv.head_stride + 8 * g);
         const uint8_t * zeros = reinterpret_cast<const uint8_t *>(pa_zeros);
 
-        // lanes l and l + 16 look after cell l of a tile: its page one tile ahead
+        // lane l looks after cell l % TILE of a tile: its page one tile ahead
         auto page_at = [&](int32_t i, int32_t & pos) {
-            pos = lo + i * PA_TILE + (lane & 15);
+            pos = lo + i * TILE + (lane & (TILE - 1));
             if (i >= n || pos >= hi) { pos = -1; return 0; }
             return __ldg(table + page_of(a.kv, pos));
         };
@@ -411,26 +414,30 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                 }
             }
         }
-        uint4 K[2][KL], V[4][VH];
-        bool ok[4];
+        uint4 K[SUB][2][KL], V[SUB][4][VH];
+        bool ok[SUB][4];
         auto load_k = [&](uint32_t off) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t f = __shfl_sync(0xffffffffu, off, g + 8 * u);
-                const uint8_t * p = f != 0xffffffffu ? kb + (uint64_t)f * a.kv.unit_bytes : zeros;
+            for (int b = 0; b < SUB; ++b)
 #pragma unroll
-                for (int i = 0; i < KL; ++i) K[u][i] = pa_load(reinterpret_cast<const uint16_t *>(p) + 32 * i);
-            }
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t f = __shfl_sync(0xffffffffu, off, 16 * b + g + 8 * u);
+                    const uint8_t * p = f != 0xffffffffu ? kb + (uint64_t)f * a.kv.unit_bytes : zeros;
+#pragma unroll
+                    for (int i = 0; i < KL; ++i) K[b][u][i] = pa_load(reinterpret_cast<const uint16_t *>(p) + 32 * i);
+                }
         };
         auto load_v = [&](uint32_t off) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint32_t f = __shfl_sync(0xffffffffu, off, 2 * t + (u & 1) + 4 * (u & 2));
-                ok[u] = f != 0xffffffffu;
-                const uint8_t * p = ok[u] ? vb + (uint64_t)f * a.kv.unit_bytes : zeros;
+            for (int b = 0; b < SUB; ++b)
 #pragma unroll
-                for (int h = 0; h < VH; ++h) V[u][h] = pa_load(reinterpret_cast<const uint16_t *>(p) + 64 * h);
-            }
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t f = __shfl_sync(0xffffffffu, off, 16 * b + 2 * t + (u & 1) + 4 * (u & 2));
+                    ok[b][u] = f != 0xffffffffu;
+                    const uint8_t * p = ok[b][u] ? vb + (uint64_t)f * a.kv.unit_bytes : zeros;
+#pragma unroll
+                    for (int h = 0; h < VH; ++h) V[b][u][h] = pa_load(reinterpret_cast<const uint16_t *>(p) + 64 * h);
+                }
         };
         uint32_t off = offset_of(page, pos);
         load_k(off);
@@ -475,33 +482,40 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             for (int j = 0; j < 8; ++j) o[h][j][0] = o[h][j][1] = 0.0f;
 
         for (int32_t i = warp; i < n; i += PA_WARPS) {
-            float s[2][4];
+            float x[SUB][4];   // scores of cells 16 b + 2t, 2t + 1, 2t + 8, 2t + 9
+            float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int b = 0; b < SUB; ++b) {
+                float s[2][4];
 #pragma unroll
-                for (int k = 0; k < KL; ++k) {
-                    if (k == 0) pa_mma0<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], K[u][k].x, K[u][k].y);
-                    else        pa_mma<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], K[u][k].x, K[u][k].y);
-                    pa_mma<BF16>(s[u], qh[k][2], qm[k][2], qh[k][3], qm[k][3], K[u][k].z, K[u][k].w);
-                    if (BF16 && !FOUR) {
-                        pa_mma<BF16>(s[u], ql[k][0], 0u, ql[k][1], 0u, K[u][k].x, K[u][k].y);
-                        pa_mma<BF16>(s[u], ql[k][2], 0u, ql[k][3], 0u, K[u][k].z, K[u][k].w);
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int k = 0; k < KL; ++k) {
+                        const uint4 & w = K[b][u][k];
+                        if (k == 0) pa_mma0<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], w.x, w.y);
+                        else        pa_mma<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], w.x, w.y);
+                        pa_mma<BF16>(s[u], qh[k][2], qm[k][2], qh[k][3], qm[k][3], w.z, w.w);
+                        if (BF16 && !FOUR) {
+                            pa_mma<BF16>(s[u], ql[k][0], 0u, ql[k][1], 0u, w.x, w.y);
+                            pa_mma<BF16>(s[u], ql[k][2], 0u, ql[k][3], 0u, w.z, w.w);
+                        }
                     }
                 }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[b][u] = s[u >> 1][u & 1] + s[u >> 1][2 + (u & 1)];
             }
             // the next tile's K comes while this tile's softmax and values are worked on
             off = offset_of(page2, pos2);
             load_k(off);
             page2 = page_at(i + 2 * PA_WARPS, pos2);
 
-            float x[4];   // cells 2t, 2t + 1, 2t + 8, 2t + 9
-            float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                x[u] = s[u >> 1][u & 1] + s[u >> 1][2 + (u & 1)];
-                if (FOUR) x[u] += __shfl_xor_sync(0xffffffffu, x[u], 16);   // the parts in rows g and g + 4
-                top = fmaxf(top, ok[u] ? __fmul_rn(x[u], c) : -INFINITY);
-            }
+            for (int b = 0; b < SUB; ++b)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (FOUR) x[b][u] += __shfl_xor_sync(0xffffffffu, x[b][u], 16);   // the parts in rows g and g + 4
+                    top = fmaxf(top, ok[b][u] ? __fmul_rn(x[b][u], c) : -INFINITY);
+                }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float mn = fmaxf(m, ceilf(top));
@@ -511,31 +525,37 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             // one rounding from the score on, as long as the maximum of the rounded products is
             // within 2^-8 of the exact ones' (2^16 has steps of 2^-7); the rounded products beyond
             const bool big = !(fabsf(base) < 65536.0f);
+            l *= fix;
+            uint32_t ph[SUB][2], pm[SUB][2], pl[SUB][2];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                x[u] = !ok[u] ? 0.0f : pa_ex2(big ? __fmul_rn(x[u], c) - base + PA_SHIFT : fmaf(x[u], c, PA_SHIFT - base));
-            l = fmaf(l, fix, (x[0] + x[1]) + (x[2] + x[3]));
-            uint32_t h0, m0, l0, h1, m1, l1;
-            pa_split<BF16>(x[0], x[1], h0, m0, l0);
-            pa_split<BF16>(x[2], x[3], h1, m1, l1);
-            if (FOUR) {
-                h0 = g < 4 ? h0 : m0;
-                h1 = g < 4 ? h1 : m1;
-                m0 = g < 4 ? l0 : 0u;
-                m1 = g < 4 ? l1 : 0u;
+            for (int b = 0; b < SUB; ++b) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    x[b][u] = !ok[b][u] ? 0.0f : pa_ex2(big ? __fmul_rn(x[b][u], c) - base + PA_SHIFT : fmaf(x[b][u], c, PA_SHIFT - base));
+                l += (x[b][0] + x[b][1]) + (x[b][2] + x[b][3]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    pa_split<BF16>(x[b][2 * u], x[b][2 * u + 1], ph[b][u], pm[b][u], pl[b][u]);
+                    if (FOUR) {
+                        ph[b][u] = g < 4 ? ph[b][u] : pm[b][u];
+                        pm[b][u] = g < 4 ? pl[b][u] : 0u;
+                    }
+                }
             }
 #pragma unroll
             for (int h = 0; h < VH; ++h) {
-                const uint32_t * va = reinterpret_cast<const uint32_t *>(&V[0][h]), * vc = reinterpret_cast<const uint32_t *>(&V[1][h]);
-                const uint32_t * vd = reinterpret_cast<const uint32_t *>(&V[2][h]), * ve = reinterpret_cast<const uint32_t *>(&V[3][h]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-                    const uint32_t b0 = __byte_perm(va[j >> 1], vc[j >> 1], sel);
-                    const uint32_t b1 = __byte_perm(vd[j >> 1], ve[j >> 1], sel);
                     float r[4];
-                    pa_mma0<BF16>(r, h0, m0, h1, m1, b0, b1);
-                    if (BF16 && !FOUR) pa_mma<BF16>(r, l0, 0u, l1, 0u, b0, b1);
+#pragma unroll
+                    for (int b = 0; b < SUB; ++b) {
+                        auto word = [&](int u) { return reinterpret_cast<const uint32_t *>(&V[b][u][h])[j >> 1]; };
+                        const uint32_t b0 = __byte_perm(word(0), word(1), sel), b1 = __byte_perm(word(2), word(3), sel);
+                        if (b == 0) pa_mma0<BF16>(r, ph[b][0], pm[b][0], ph[b][1], pm[b][1], b0, b1);
+                        else        pa_mma<BF16>(r, ph[b][0], pm[b][0], ph[b][1], pm[b][1], b0, b1);
+                        if (BF16 && !FOUR) pa_mma<BF16>(r, pl[b][0], 0u, pl[b][1], 0u, b0, b1);
+                    }
                     o[h][j][0] = fmaf(o[h][j][0], fix, r[0] + r[2]);
                     o[h][j][1] = fmaf(o[h][j][1], fix, r[1] + r[3]);
                 }
@@ -604,7 +624,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
                     for (int e = 0; e < N; e += 4)
                         *reinterpret_cast<float4 *>(&piece->o[h][d + e]) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-                    if ((tid & 15) == 0) { piece->m[h] = M; piece->l[h] = Ls; }
+                    if ((tid & 15) == 0) { a.meta->m[begins][h][cta] = M; a.meta->l[begins][h][cta] = Ls; }
                 }
             }
             if (!begins) head_ends = ends;
@@ -615,7 +635,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         tile = 0;
         if (left > 0 && ++unit == units) {
             unit = 0;
-            do ++row; while (pa_tiles(a, row) == 0);
+            do ++row; while (pa_tiles<TILE>(a, row) == 0);
         }
     }
     if (tid == 0) {
@@ -660,14 +680,14 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
         const int i = i0 + 4 * lane + part;
         m = -INFINITY;
         l = 0.0f;
-        if (cta + i < grid) { m = piece(i)->m[h]; l = piece(i)->l[h]; }
+        if (cta + i < grid) { m = a.meta->m[i == 0][h][cta + i]; l = a.meta->l[i == 0][h][cta + i]; }
         last = ends[0] ? 0 : ends[1] ? 1 : ends[2] ? 2 : ends[3] ? 3 : 4;
     };
     const int32_t row = a.meta->tail_row[cta], unit = a.meta->tail_unit[cta];
+    look(0);
     const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
     const int heads = min(8, a.G - 8 * grp);
     if (row >= 0 && PJ_HEADS * (int)blockIdx.y < heads) {   // uniform over the block
-        look(0);
         float M = -INFINITY, L = 0.0f, acc[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] = 0.0f;
@@ -809,7 +829,7 @@ size_t attn_ws_bytes(int D) {
 
 template <int D, bool BF16>
 cudaError_t launch_attn(const PaArgs & a, cudaStream_t st) {
-    const int ctas = min(PA_MAX_CTAS, PA_CTAS_PER_SM<D> * alb_sm_count());
+    const int ctas = min(PA_MAX_CTAS, PA_CTAS_PER_SM * alb_sm_count());
     auto * f = BF16 && a.G <= 4 ? k_paged_attn<D, BF16, BF16> : k_paged_attn<D, BF16, false>;
     cudaError_t e = alb_launch(f, dim3((unsigned)ctas), dim3(PA_THREADS), 0, st, true, a);
     if (e != cudaSuccess) return e;
