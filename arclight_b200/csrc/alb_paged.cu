@@ -241,7 +241,15 @@ __device__ __forceinline__ float pa_ex2(float x) {
 }
 __device__ const uint4 pa_zeros[16] = {};   // what a cell that is not seen reads instead
 
-__device__ __forceinline__ uint4 pa_load(const uint16_t * p) {
+// 16 bytes of K: an instruction takes 64 bytes from each of 8 cells, so its line
+// stays in the L1 cache for the next one.
+__device__ __forceinline__ uint4 pa_load_k(const uint16_t * p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::evict_first.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+// 16 bytes of V: an instruction takes whole lines.
+__device__ __forceinline__ uint4 pa_load_v(const uint16_t * p) {
     uint4 r;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
@@ -424,7 +432,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                     const uint32_t f = __shfl_sync(0xffffffffu, off, 16 * b + g + 8 * u);
                     const uint8_t * p = f != 0xffffffffu ? kb + (uint64_t)f * a.kv.unit_bytes : zeros;
 #pragma unroll
-                    for (int i = 0; i < KL; ++i) K[b][u][i] = pa_load(reinterpret_cast<const uint16_t *>(p) + 32 * i);
+                    for (int i = 0; i < KL; ++i) K[b][u][i] = pa_load_k(reinterpret_cast<const uint16_t *>(p) + 32 * i);
                 }
         };
         auto load_v = [&](uint32_t off) {
@@ -436,7 +444,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                     ok[b][u] = f != 0xffffffffu;
                     const uint8_t * p = ok[b][u] ? vb + (uint64_t)f * a.kv.unit_bytes : zeros;
 #pragma unroll
-                    for (int h = 0; h < VH; ++h) V[b][u][h] = pa_load(reinterpret_cast<const uint16_t *>(p) + 64 * h);
+                    for (int h = 0; h < VH; ++h) V[b][u][h] = pa_load_v(reinterpret_cast<const uint16_t *>(p) + 64 * h);
                 }
         };
         uint32_t off = offset_of(page, pos);
