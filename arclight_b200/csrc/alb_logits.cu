@@ -11,6 +11,8 @@
 // bias and penalties applied, and what is left for the one pass over the logits
 // is the same for every token: the settled value where there is one, temperature,
 // mask, maximum.  The CTAs' maxima go to CTA 0's shared memory.
+#include <atomic>
+
 #include "alb_common.cuh"
 #include "alb_internal.h"
 
@@ -23,7 +25,7 @@ constexpr int LG_WARPS = LG_THREADS / 32;
 constexpr int LG_BATCH = 3;              // 16-byte loads of logits in flight per thread
 constexpr int LG_GRANULE = 128;          // tokens dealt out together: a group of four per lane of a warp
 constexpr int LG_MAX_CLUSTER = 16;
-constexpr int LG_LIST = 1024;            // ids of a CTA whose settled values it holds
+constexpr int LG_LIST = 2048;            // ids of a CTA whose settled values it holds
 
 // A table entry: how often the id is in the counted output, and two marks (the
 // id is in the prompt; its logit with bias waits in y), until the id is settled:
@@ -33,7 +35,7 @@ template <typename T> struct Entry {
     static constexpr uint32_t PROMPT = 1u << (8 * sizeof(T) - 1), BIASED = PROMPT >> 1, COUNT = BIASED - 1;
 };
 
-constexpr size_t LG_STATIC = 8192;                  // bound of the kernel's static shared memory
+constexpr size_t LG_STATIC = 16384;                 // bound of the kernel's static shared memory
 
 struct LogitsArgs {
     const float * x;
@@ -432,9 +434,14 @@ template <typename T, bool TABLE>
 cudaError_t launch_logits(const LogitsArgs & a, int64_t rows, cudaStream_t st) {
     const size_t smem = (size_t)a.granules * LG_GRANULE * (TABLE ? sizeof(T) : 0) + (a.r.allow ? (size_t)a.granules * 16 : 0);
     const unsigned cluster = 1u << a.log_cluster;
+    static std::atomic<bool> wide_clusters[64];   // per device: clusters of 16 are allowed
     cudaError_t e = ensure_smem(k_logits<T, TABLE>, smem + LG_STATIC);   // the limit holds for both kinds together
-    if (e == cudaSuccess && cluster > 8)
+    int dev = 0;
+    if (e == cudaSuccess && cluster > 8) e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && cluster > 8 && (dev >= 64 || !wide_clusters[dev].load(std::memory_order_acquire))) {
         e = cudaFuncSetAttribute(k_logits<T, TABLE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess && dev < 64) wide_clusters[dev].store(true, std::memory_order_release);
+    }
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster));
@@ -483,8 +490,13 @@ extern "C" int alb_logits_process(const float * logits, int64_t rows, int64_t n_
     const int64_t most = r.last_n > 0 && r.last_n < a.r.history_stride ? r.last_n : a.r.history_stride;
     const bool wide = most >= (1 << 14);
     const int64_t granules = (n_vocab + 3 + LG_GRANULE - 1) / LG_GRANULE;   // + 3: the first place may lie before the row
-    const int64_t share = !table ? 0 : LG_GRANULE * (wide ? 4 : 2);
-    a.log_cluster = rows <= 8 || granules * share > 8 * 65536 ? 4 : 3;
+    // CTAs per row: enough that a share is at most 20000 tokens (its table leaves room for three CTAs an SM);
+    // more while the rows do not fill the SMs and a share is worth a CTA's fixed cost
+    const int64_t room = wide ? 10000 : 20000;
+    a.log_cluster = 0;
+    while (a.log_cluster < 4 && ((n_vocab >> a.log_cluster) > room ||
+                                 ((rows << a.log_cluster) < alb_sm_count() && (n_vocab >> a.log_cluster) > 4096)))
+        ++a.log_cluster;
     a.granules = (int32_t)((granules + (1 << a.log_cluster) - 1) >> a.log_cluster);
     a.err = device_error_ptr();
     ALB_CUDA_TRY(a.err ? cudaSuccess : cudaErrorMemoryAllocation);

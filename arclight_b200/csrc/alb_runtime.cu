@@ -50,12 +50,13 @@ cudaError_t ensure_dynamic_smem(const void * func, size_t bytes) {
 }
 
 int * device_error_ptr() {
-    static int * ptrs[64] = {nullptr};
+    static std::atomic<int *> ptrs[64];
     static std::mutex mu;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (int * known = ptrs[dev].load(std::memory_order_acquire)) return known;
     std::lock_guard<std::mutex> lk(mu);
-    if (!ptrs[dev]) {
+    if (!ptrs[dev].load(std::memory_order_relaxed)) {
         // Once per device, never on the hot path.  The first call may come while a
         // stream is being captured: the relaxed mode lets this thread allocate
         // then, and the zeroing runs on a stream of its own.
@@ -69,9 +70,9 @@ int * device_error_ptr() {
         if (!ok && p) cudaFree(p);
         cudaThreadExchangeStreamCaptureMode(&mode);
         if (!ok) return nullptr;
-        ptrs[dev] = p;
+        ptrs[dev].store(p, std::memory_order_release);
     }
-    return ptrs[dev];
+    return ptrs[dev].load(std::memory_order_relaxed);
 }
 }  // namespace alb
 
