@@ -23,6 +23,7 @@ namespace {
 constexpr int LG_THREADS = 512;
 constexpr int LG_WARPS = LG_THREADS / 32;
 constexpr int LG_BATCH = 3;              // 16-byte loads of logits in flight per thread
+constexpr int LG_IDS = 4;                // loads of ids in flight per thread
 constexpr int LG_GRANULE = 128;          // tokens dealt out together: a group of four per lane of a warp
 constexpr int LG_MAX_CLUSTER = 16;
 constexpr int LG_LIST = 2048;            // ids of a CTA whose settled values it holds
@@ -265,24 +266,13 @@ k_logits(const __grid_constant__ LogitsArgs a) {
                     if (at < LG_LIST) list[at] = (uint16_t)j;
                 }
             };
-            int32_t e = start + tid;
-            for (; e + 7 * LG_THREADS < len; e += 8 * LG_THREADS) {
-                int32_t id[8];
+            for (int32_t e = start + tid; e < len; e += LG_IDS * LG_THREADS) {
+                int32_t id[LG_IDS];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) id[u] = h[e + u * LG_THREADS];
+                for (int u = 0; u < LG_IDS; ++u) id[u] = e + u * LG_THREADS < len ? h[e + u * LG_THREADS] : -1;
 #pragma unroll
-                for (int u = 0; u < 8; ++u) count(e + u * LG_THREADS, id[u]);
-            }
-            if (e < len) {
-                int32_t id[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) id[u] = e + u * LG_THREADS < len ? h[e + u * LG_THREADS] : -1;
-#pragma unroll 1
-                for (int u = 0; u < 8 && e < len; ++u, e += LG_THREADS) {
-                    count(e, id[0]);
-#pragma unroll
-                    for (int w = 0; w < 7; ++w) id[w] = id[w + 1];
-                }
+                for (int u = 0; u < LG_IDS; ++u)
+                    if (e - tid + u * LG_THREADS < len) count(e + u * LG_THREADS, id[u]);
             }
         }
         __syncthreads();   // every id is counted
