@@ -55,7 +55,7 @@ template <> struct Vec<4> { using F = float4; };
 // its order.  The four sums are folded together (half the lanes keep two of them,
 // a quarter one): 6 exchanges instead of 20, and the eight lanes that end with a
 // head's sum find its scale, all four heads at once.
-constexpr int AP_HEADS = 4, AP_WARPS = 4;
+constexpr int AP_HEADS = 4, AP_WARPS = 2;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(32 * AP_WARPS)
 k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int Hq, const float * __restrict__ qn_w,
