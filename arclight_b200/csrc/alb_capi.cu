@@ -82,7 +82,7 @@ void rope_table_host(std::vector<float> & t, int32_t max_pos, int32_t head_dim, 
 }  // namespace alb
 
 extern "C" int alb_rope_table(float * table_dev, int32_t max_pos, int32_t head_dim, float freq_base) {
-    ALB_CHECK_ARG(table_dev && max_pos > 0 && head_dim == 128 && freq_base > 0.0f);
+    ALB_CHECK_ARG(table_dev && max_pos > 0 && (head_dim == 64 || head_dim == 128) && freq_base > 0.0f);
     std::vector<float> t;
     rope_table_host(t, max_pos, head_dim, freq_base);
     ALB_CUDA_TRY(cudaMemcpy(table_dev, t.data(), t.size() * sizeof(float), cudaMemcpyHostToDevice));

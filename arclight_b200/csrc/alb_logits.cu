@@ -468,6 +468,10 @@ extern "C" int alb_logits_process(const float * logits, int64_t rows, int64_t n_
     ALB_CHECK_ARG(r.last_n >= 0);
     ALB_CHECK_ARG(!r.bias_ids || (r.bias_values && r.bias_offsets && r.n_bias >= 0 && r.n_bias < (1 << 30)));
     ALB_CHECK_ARG(!r.allow || (r.n_allow > 0 && (r.allow_stride == 0 || r.allow_stride >= (n_vocab + 31) / 32)));
+    ALB_CHECK_ARG((((uintptr_t)next_token | (uintptr_t)r.history | (uintptr_t)r.history_len | (uintptr_t)r.prompt_len |
+                    (uintptr_t)r.repetition | (uintptr_t)r.frequency | (uintptr_t)r.presence | (uintptr_t)r.temperature |
+                    (uintptr_t)r.bias_offsets | (uintptr_t)r.bias_ids | (uintptr_t)r.bias_values | (uintptr_t)r.allow |
+                    (uintptr_t)r.allow_row) & 3) == 0);
     LogitsArgs a = {};
     a.x = logits; a.y = out; a.n_vocab = n_vocab; a.x_stride = xs; a.y_stride = ys; a.next = next_token; a.r = r;
     if (!r.repetition && !r.frequency && !r.presence) a.r.history = nullptr;   // nothing asks for the counts

@@ -158,9 +158,9 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // tensor cores (mma m16n8k16, fp32 accumulators), everything in registers.
 //
 // A unit is (row, K/V head, group of up to 8 query heads).  Its cells come in
-// tiles of 16 (D = 128) or 32, and all tiles of all units form one line that is cut into equal
-// ranges, one per CTA (k_paged_attn): uneven lengths and few rows load the SMs
-// alike, and nothing depends on the lengths but device code.  In a CTA's
+// tiles of 16 (D = 128) or 32, and all tiles of all units, each unit's led by a
+// few that stand for its setup, form one line that is cut into equal ranges, one
+// per CTA (k_paged_attn): uneven lengths and few rows load the SMs alike, and nothing depends on the lengths but device code.  In a CTA's
 // segment of a unit warp w takes every fourth tile; the warps join through
 // shared memory, and the pieces of a unit that a range's border cuts are joined
 // by k_paged_attn_join.
@@ -190,6 +190,7 @@ constexpr int PA_CTAS_PER_SM = 3;        // what the registers allow (168 a thre
 template <int D> constexpr int PA_TILE = 16 * 128 / D;
 constexpr int PA_MAX_CTAS = 1024;
 constexpr int PA_MIN_TILES = 4;          // a CTA's range is at least a tile per warp
+constexpr int PA_SETUP = 6;              // what a unit costs beside its tiles, in tiles
 constexpr float PA_SHIFT = 15.0f;
 
 // What each CTA left unfinished: the unit that its range began and did not end
@@ -232,6 +233,12 @@ template <int TILE> __device__ __forceinline__ int32_t pa_tiles(const PaArgs & a
     bool bad;
     pa_span(a, r, lo, hi, seq, bad);
     return (int32_t)(((uint32_t)(hi - lo) + TILE - 1) / TILE);
+}
+
+// What a unit of row r weighs on the line: its tiles, and the work that any unit is.
+template <int TILE> __device__ __forceinline__ int32_t pa_weight(const PaArgs & a, int64_t r) {
+    const int32_t n = pa_tiles<TILE>(a, r);
+    return n ? n + PA_SETUP : 0;
 }
 
 __device__ __forceinline__ float pa_ex2(float x) {
@@ -319,7 +326,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
     const int64_t per_thread = (a.n_rows + PA_THREADS - 1) / PA_THREADS;
     const int64_t r0 = tid * per_thread, r1 = min(a.n_rows, r0 + per_thread);
     int64_t mine = 0;
-    for (int64_t r = r0; r < r1; ++r) mine += pa_tiles<TILE>(a, r);
+    for (int64_t r = r0; r < r1; ++r) mine += pa_weight<TILE>(a, r);
     int64_t scan = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -348,14 +355,14 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         int64_t rem = start - before;
         int64_t r = r0;
         for (;; ++r) {
-            const int64_t here = (int64_t)pa_tiles<TILE>(a, r) * units;
+            const int64_t here = (int64_t)pa_weight<TILE>(a, r) * units;
             if (rem < here) break;
             rem -= here;
         }
-        const int32_t n = pa_tiles<TILE>(a, r);
+        const int32_t n = pa_weight<TILE>(a, r);
         at_row = (int32_t)r;
         at_unit = (int32_t)(rem / n);
-        at_tile = (int32_t)(rem % n);
+        at_tile = (int32_t)(rem % n) - PA_SETUP;
     }
     __syncthreads();
     int32_t tail_row = -1, tail_unit = 0, head_ends = 0;
@@ -380,9 +387,12 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         bool bad;
         pa_span(a, row, lo, hi, seq, bad);
         const int32_t all = (int32_t)(((uint32_t)(hi - lo) + TILE - 1) / TILE);
-        const int32_t n = (int32_t)min((int64_t)(all - tile), left);
-        const bool begins = tile == 0, ends = tile + n == all;
-        lo += tile * TILE;
+        const int32_t take = (int32_t)min((int64_t)(all - tile), left);
+        left -= take;
+        if (tile + take <= 0) break;         // the range ends in the unit's setup, which is the next one's then
+        const bool begins = tile <= 0, ends = tile + take == all;
+        const int32_t n = begins ? tile + take : take;
+        lo += max(tile, 0) * TILE;
         const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
         const int heads = min(8, a.G - 8 * grp);
         const int32_t head0 = kvh * a.G + 8 * grp;
@@ -639,8 +649,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             else if (!ends) { tail_row = row; tail_unit = unit; }
         }
         __syncthreads();   // the shared sums are free again
-        left -= n;
-        tile = 0;
+        tile = -PA_SETUP;
         if (left > 0 && ++unit == units) {
             unit = 0;
             do ++row; while (pa_tiles<TILE>(a, row) == 0);
@@ -657,8 +666,8 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 // not end: its tail, then the heads of the CTAs behind it up to the one that ends
 // the unit.  A block takes two of the unit's heads, a head four warps, a warp
 // every fourth piece and a lane D/32 neighbouring values.  What tells whether
-// there is work, where it ends and what the pieces weigh is loaded at once, 128
-// pieces a round; the pieces' maxima are whole numbers, so rescaling is exact
+// there is work, where it ends and what the pieces weigh is loaded at once, 32
+// pieces a warp and round; the pieces' maxima are whole numbers, so rescaling is exact
 // whatever the order.
 constexpr int PJ_HEADS = 2, PJ_PARTS = 4, PJ_THREADS = 32 * PJ_HEADS * PJ_PARTS;
 template <int D>
@@ -674,22 +683,25 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
     const PaPiece<D> * pieces = static_cast<const PaPiece<D> *>(a.pieces);
     // piece i: the tail of this CTA, then the head of the i-th CTA behind it
     auto piece = [&](int i) { return pieces + 2 * (cta + i) + (i == 0 ? 1 : 0); };
-    // lane l looks after pieces 4 l .. 4 l + 3 of a round for where the unit ends, after 4 l + part for its weight
-    static_assert(PJ_PARTS == 4, "four pieces per lane");
-    int last;                 // place of the first end among this lane's four, or 4
+    // lane l looks after pieces PARTS l .. of a round for where the unit ends, after PARTS l + part for its weight
+    int last;                 // place of the first end among this lane's, or PARTS
     float m, l;
     auto look = [&](int i0) {
-        int ends[4];
+        int ends[PJ_PARTS];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int c = cta + i0 + 4 * lane + u;
-            ends[u] = c >= grid - 1 ? 1 : i0 + lane + u > 0 ? a.meta->head_ends[c] : 0;
+        for (int u = 0; u < PJ_PARTS; ++u) {
+            const int c = cta + i0 + PJ_PARTS * lane + u;
+            ends[u] = a.meta->head_ends[min(c, grid - 1)] | (c >= grid - 1);
+            if (i0 + lane + u == 0) ends[u] = 0;   // the tail itself (CTA `cta`; a last CTA has none)
         }
-        const int i = i0 + 4 * lane + part;
+        last = PJ_PARTS;
+#pragma unroll
+        for (int u = PJ_PARTS - 1; u >= 0; --u)
+            if (ends[u]) last = u;
+        const int i = i0 + PJ_PARTS * lane + part;
         m = -INFINITY;
         l = 0.0f;
         if (cta + i < grid) { m = a.meta->m[i == 0][h][cta + i]; l = a.meta->l[i == 0][h][cta + i]; }
-        last = ends[0] ? 0 : ends[1] ? 1 : ends[2] ? 2 : ends[3] ? 3 : 4;
     };
     const int32_t row = a.meta->tail_row[cta], unit = a.meta->tail_unit[cta];
     look(0);
@@ -701,10 +713,10 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
         for (int e = 0; e < N; ++e) acc[e] = 0.0f;
         if (h < heads) {
             for (int i0 = 0;;) {
-                const uint32_t e = __ballot_sync(0xffffffffu, last < 4);
+                const uint32_t e = __ballot_sync(0xffffffffu, last < PJ_PARTS);
                 const int who = e ? __ffs(e) - 1 : 31;
-                const int n = e ? 4 * who + __shfl_sync(0xffffffffu, last, who) + 1 : 128;   // pieces of this round
-                if (4 * lane + part >= n) { m = -INFINITY; l = 0.0f; }
+                const int n = e ? PJ_PARTS * who + __shfl_sync(0xffffffffu, last, who) + 1 : 32 * PJ_PARTS;   // pieces of this round
+                if (PJ_PARTS * lane + part >= n) { m = -INFINITY; l = 0.0f; }
                 const float Mn = fmaxf(M, alb_warp_max(m)), base = Mn == -INFINITY ? 0.0f : Mn;
                 const float fix = pa_ex2(M - base), f = pa_ex2(m - base);
                 L = fmaf(L, fix, alb_warp_sum(l * f));
@@ -712,15 +724,15 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
                 for (int k = 0; k < N; ++k) acc[k] *= fix;
                 M = Mn;
 #pragma unroll 8
-                for (int k = 0; 4 * k + part < n; ++k) {
+                for (int k = 0; PJ_PARTS * k + part < n; ++k) {
                     const float w = __shfl_sync(0xffffffffu, f, k);
                     float v[N];
-                    *reinterpret_cast<F *>(v) = *reinterpret_cast<const F *>(&piece(i0 + 4 * k + part)->o[h][N * lane]);
+                    *reinterpret_cast<F *>(v) = *reinterpret_cast<const F *>(&piece(i0 + PJ_PARTS * k + part)->o[h][N * lane]);
 #pragma unroll
                     for (int j = 0; j < N; ++j) acc[j] = fmaf(v[j], w, acc[j]);
                 }
                 if (e) break;
-                i0 += 128;
+                i0 += 32 * PJ_PARTS;
                 look(i0);
             }
         }
@@ -769,9 +781,11 @@ bool paged_view(const alb_paged_kv * c, PagedView & kv, bool table) {
     else if (c->type != ALB_KV_F16 && c->type != ALB_KV_BF16) why = "invalid argument: paged cache type";
     else if (c->n_pages <= 0 || c->page_size <= 0 || c->n_head_kv <= 0 || c->n_seqs <= 0 || c->max_pages <= 0)
         why = "invalid argument: paged cache with an empty axis";
-    else if (c->n_pages >= ((int64_t)1 << 31) || c->n_pages * c->page_size >= ((int64_t)1 << 31) ||
-             (int64_t)c->max_pages * c->page_size >= ((int64_t)1 << 31) || c->n_head_kv > 65535)
+    else if (c->n_pages >= ((int64_t)1 << 31) || c->n_pages * c->page_size >= ((int64_t)1 << 31) || c->n_head_kv > 65535)
         why = "invalid argument: paged cache of 2^31 cells or more, or more than 65535 heads";
+    else if ((int64_t)c->max_pages * c->page_size > (1 << 30))   // (positions of a tile that starts below stay below 2^31)
+        why = "invalid argument: page table of more than 2^30 positions";
+    else if ((uintptr_t)c->page_table & 3) why = "invalid argument: page table not 4-byte aligned";
     else if (c->table_stride != 0 && (c->table_stride < c->max_pages || c->table_stride >= ((int64_t)1 << 40)))
         why = "invalid argument: page table rows overlap";
     if (why) { alb_set_last_error_msg(why); return false; }
@@ -858,6 +872,7 @@ extern "C" int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, 
     const int64_t dense = (int64_t)(n_head + 2 * v.Hkv) * kv->head_dim;
     ALB_CHECK_ARG(qkv_stride == 0 || (qkv_stride >= dense && qkv_stride % 4 == 0 && qkv_stride < ((int64_t)1 << 31)));
     ALB_CHECK_ARG((((uintptr_t)qkv | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)rope_table | (uintptr_t)q_out) & 15) == 0);
+    ALB_CHECK_ARG((((uintptr_t)positions | (uintptr_t)seqs) & 3) == 0);
     int * err = device_error_ptr();
     ALB_CUDA_TRY(err ? cudaSuccess : cudaErrorMemoryAllocation);
     auto * f = kv->head_dim == 128 ? (kv->type == ALB_KV_BF16 ? launch_append<128, true> : launch_append<128, false>)
@@ -882,6 +897,7 @@ extern "C" int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, c
     ALB_CHECK_ARG(n_head > 0 && n_head < 4096 && n_head % v.Hkv == 0);   // 2^24 rows x 2^27 tiles x 2^12 units < 2^63
     ALB_CHECK_ARG(scale > 0.0f && std::isfinite(scale));
     ALB_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0);
+    ALB_CHECK_ARG((((uintptr_t)lengths | (uintptr_t)seqs | (uintptr_t)lse) & 3) == 0);
     PaArgs a = {};
     a.q = q; a.kv = v; a.seqs = seqs; a.lengths = lengths; a.n_rows = n_rows; a.Hq = n_head; a.G = n_head / v.Hkv;
     a.groups = (a.G + 7) / 8; a.window = window; a.scale_log2 = scale * 1.44269504f; a.out = out; a.lse = lse;

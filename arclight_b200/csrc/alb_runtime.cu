@@ -41,11 +41,15 @@ cudaError_t ensure_dynamic_smem(const void * func, size_t bytes) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    std::lock_guard<std::mutex> lk(mu);
-    size_t & cur = done[std::make_pair(dev, func)];
-    if (cur >= bytes) return cudaSuccess;
-    e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) cur = bytes;
+    try {   // (the callers are C entry points)
+        std::lock_guard<std::mutex> lk(mu);
+        size_t & cur = done[std::make_pair(dev, func)];
+        if (cur >= bytes) return cudaSuccess;
+        e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess) cur = bytes;
+    } catch (...) {
+        return cudaErrorMemoryAllocation;
+    }
     return e;
 }
 

@@ -140,7 +140,8 @@ ALB_API int alb_set_rows_f16(const float * src, int64_t n_rows, int64_t row_len,
 ALB_API int alb_get_rows_f16(const uint16_t * src, int64_t src_rows, int64_t row_len, const int64_t * idx,
                              int64_t n_rows, uint16_t * dst, void * stream);
 /* RoPE cos/sin table of nnml_rope_cache_init (ops.cpp:759-771; NEOX, ext_factor 0,
- * freq_scale 1): host-computed, copied to table_dev [max_pos][head_dim/2] (cos, sin). */
+ * freq_scale 1): host-computed, copied to table_dev [max_pos][head_dim/2] (cos, sin);
+ * head_dim 64 or 128. */
 ALB_API int alb_rope_table(float * table_dev, int32_t max_pos, int32_t head_dim, float freq_base);
 /* Per-head QK-RMSNorm * w + NEOX RoPE of Q and K and the fp16 KV store of K and V
  * (qwen3.cpp:215-224, ops.cpp:830-938, set_rows ops.cpp:135-181).  qkv [T][(Hq+2Hkv)*128]
@@ -221,7 +222,7 @@ typedef struct {
     int64_t         head_stride;
     int64_t         n_pages;      /* n_pages * page_size < 2^31 */
     int32_t         n_seqs;
-    int32_t         max_pages;    /* max_pages * page_size < 2^31 */
+    int32_t         max_pages;    /* max_pages * page_size <= 2^30 */
     int32_t         page_size;    /* any size from 1 */
     int32_t         n_head_kv;
     int32_t         head_dim;     /* 64 or 128 */
@@ -257,7 +258,8 @@ ALB_API int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, int
  * of summation follows the lengths of the whole batch; the same call gives the
  * same bits.  A row that sees nothing (length 0) is 0, its lse -INFINITY; a row
  * with a negative length is padding and left as it was.  Cells outside a row's
- * range are not read.  A sequence outside [0, n_seqs) leaves its row without
+ * range are not read; in the cells it sees, K and V are finite (a head that meets
+ * an infinity or NaN there, or in its query, gets values that are not finite).  A sequence outside [0, n_seqs) leaves its row without
  * cells, a length beyond the table is cut to it, and the cells of a page outside
  * [0, n_pages) are not seen; each makes alb_device_error() report 4.  A prompt's
  * tokens may be rows too (their own lengths), each reading its cells anew.

@@ -35,7 +35,7 @@ BAD_CACHES = [
     dict(k=None), dict(v=None), dict(page_table=None), dict(k=P + 2), dict(v=P + 8), dict(head_dim=96),
     dict(head_dim=0), dict(type=2), dict(type=-1), dict(n_pages=0), dict(page_size=0), dict(page_size=-4),
     dict(n_head_kv=0), dict(n_seqs=0), dict(max_pages=0), dict(n_pages=1 << 31), dict(n_pages=1 << 27),
-    dict(max_pages=1 << 27), dict(table_stride=3), dict(table_stride=-4),
+    dict(max_pages=(1 << 26) + 1), dict(page_table=P + 2), dict(table_stride=3), dict(table_stride=-4),
     dict(head_stride=128),                                                    # only one of the three strides
     dict(head_stride=128, cell_stride=128, page_stride=4096),                 # cells on top of one another
     dict(head_stride=128, cell_stride=256, page_stride=4000),                 # pages on top of one another
@@ -57,7 +57,8 @@ def test_attention_refusals():
     assert attend(None) == A.ALB_ERR_INVALID
     for bad in (dict(q=None), dict(lengths=None), dict(ws=None), dict(out=None), dict(rows=0), dict(rows=1 << 24),
                 dict(heads=0), dict(heads=7), dict(heads=1), dict(window=-1), dict(scale=0.0), dict(scale=-1.0),
-                dict(scale=float("nan")), dict(scale=float("inf")), dict(q=P + 4), dict(out=P + 8), dict(ws=P + 4)):
+                dict(scale=float("nan")), dict(scale=float("inf")), dict(q=P + 4), dict(out=P + 8), dict(ws=P + 4), dict(heads=4096),
+                dict(lengths=P + 1), dict(seqs=P + 2), dict(lse=P + 2)):
         assert attend(ok, **bad) == A.ALB_ERR_INVALID, bad
     need = A.lib().alb_paged_attn_workspace_bytes
     assert need(None, 1, 8) == 0
@@ -73,7 +74,7 @@ def test_append_refusals():
     for bad in (dict(qkv=None), dict(rope=None), dict(pos=None), dict(q=None), dict(T=0), dict(T=1 << 30),
                 dict(heads=0), dict(max_pos=0), dict(eps=-1.0), dict(eps=float("nan")), dict(qkv=P + 4),
                 dict(rope=P + 8), dict(q=P + 4), dict(qn=P + 4), dict(kn=P + 2), dict(stride=12 * 128 - 4),
-                dict(stride=12 * 128 + 2)):
+                dict(stride=12 * 128 + 2), dict(pos=P + 2), dict(seqs=P + 1)):
         assert append(ok, **bad) == A.ALB_ERR_INVALID, bad
 
 
@@ -88,7 +89,8 @@ def test_logits_refusals():
                 dict(y=P + 4 * 3 * 1000), dict(history=P, repetition=P), dict(history=P, history_stride=1 << 30, presence=P),
                 dict(last_n=-1), dict(bias_ids=P, n_bias=4), dict(bias_ids=P, bias_values=P, n_bias=4),
                 dict(bias_ids=P, bias_values=P, bias_offsets=P, n_bias=-1), dict(allow=P), dict(allow=P, n_allow=2, allow_stride=31),
-                dict(vocab=(1 << 19) + 1, y=1 << 30, history=P, history_stride=4, frequency=P)):
+                dict(vocab=450001, y=1 << 30), dict(nxt=P + 2), dict(temperature=P + 1), dict(history=P + 2, history_stride=4, frequency=P),
+                dict(allow=P + 1, n_allow=2)):
         assert call(**bad) == A.ALB_ERR_INVALID, bad
 
 

@@ -315,3 +315,31 @@ def test_two_streams_and_a_replayed_graph():
     wy, wn = plain(x2, **kw)
     np.testing.assert_array_equal(ys[2].cpu().numpy(), wy)
     np.testing.assert_array_equal(ns[2].cpu().numpy(), wn)
+
+
+@pytest.mark.parametrize("vocab,hist", [(16000, 9000), (9000, 20000)])   # 16-bit and 32-bit counts
+def test_more_distinct_ids_than_a_cta_lists(vocab, hist):
+    rng = np.random.default_rng(hist)
+    x, kw = case(rng, 160, vocab, hist, 20, True)
+    kw["history"] = rng.integers(0, vocab, (160, hist)).astype(np.int32)
+    kw["lens"][:] = rng.integers(0, hist + 1, 160)
+    kw["lens"][:3] = (hist, hist, 0)
+    same(x, kw)
+    same(x, kw, inplace=True)
+
+
+def test_division_by_the_temperature_rounds_as_the_quotient():
+    """Values over all exponents, temperatures inside and outside the range of the short division."""
+    rng = np.random.default_rng(3)
+    temps = np.concatenate([rng.uniform(0.01, 3.0, 40), 2.0 ** rng.uniform(-19.9, 19.9, 20),
+                            [2.0 ** -20, 2.0 ** 20, np.nextafter(F(2.0 ** -20), F(1)), 1e-25, 1e25, 1e-42, 3e38, 1.0, 0.7, 1.9999999]]).astype(F)
+    bits = rng.integers(0, 2 ** 32, (len(temps), 30000), dtype=np.uint64).astype(np.uint32)
+    x = bits.view(F).copy()
+    x[np.isnan(x)] = 0
+    x[:, ::3] = (rng.standard_normal(x[:, ::3].shape) * 5).astype(F)
+    x[:, :6] = [0.0, -0.0, np.inf, -np.inf, np.finfo(F).max, 1e-45]
+    y, n = call(x, temp=temps)
+    with np.errstate(all="ignore"):
+        want = x / temps[:, None]
+    np.testing.assert_array_equal(y.view(np.uint32), want.view(np.uint32))
+    np.testing.assert_array_equal(n, want.argmax(1))

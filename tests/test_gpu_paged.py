@@ -321,6 +321,58 @@ def test_splits_and_many_rows(rows, longest):
     check_rows(cache, q[some], [lens[r] for r in some], out[some], lse[some], seqs=some)
 
 
+def test_batches_of_nothing():
+    """All rows empty or padding, one empty row, one row among many empty ones."""
+    gen = torch.Generator().manual_seed(1)
+    dg = torch.Generator(device="cuda").manual_seed(1)
+    table, pool = make_table([70] + [0] * 599, 16, gen)
+    cache = Cache(pool, 16, 2, 64, A.ALB_KV_BF16, table)
+    cache.fill(0, 70, dg)
+    for lens in ([0], [-1], [0] * 600, [-1, 0] * 300, [70] + [0, -1] * 299 + [0]):
+        q = torch.randn(len(lens), 4, 64, generator=dg, device="cuda")
+        out, lse = attend(cache, q, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+        check_rows(cache, q, lens, out, lse)
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first call of the library is captured into a graph."""
+    import subprocess
+    import sys
+    code = """
+import ctypes as C, torch, arclight_b200 as A
+L = A.lib()
+k = torch.zeros(4, 16, 1, 64, dtype=torch.float16, device="cuda"); v = torch.ones_like(k)
+t = torch.zeros(1, 1, dtype=torch.int32, device="cuda"); n = torch.full((1,), 3, dtype=torch.int32, device="cuda")
+q = torch.ones(1, 2, 64, device="cuda"); o = torch.zeros_like(q); x = torch.ones(1, 9, device="cuda"); y = torch.zeros_like(x)
+c = A.PagedKV(k=k.data_ptr(), v=v.data_ptr(), page_table=t.data_ptr(), n_pages=4, n_seqs=1, max_pages=1, page_size=16,
+              n_head_kv=1, head_dim=64, type=A.ALB_KV_F16)
+ws = torch.empty(L.alb_paged_attn_workspace_bytes(C.byref(c), 1, 2), dtype=torch.uint8, device="cuda")
+r = A.LogitsRules(temperature=x.data_ptr())
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    A.check(L.alb_paged_attn(q.data_ptr(), 1, 2, C.byref(c), None, n.data_ptr(), 0, 0.1, ws.data_ptr(), o.data_ptr(), None, s))
+    A.check(L.alb_logits_process(x.data_ptr(), 1, 9, 0, C.byref(r), y.data_ptr(), 0, None, s))
+g.replay(); torch.cuda.synchronize()
+assert torch.all(o == 1) and torch.all(y == 1) and L.alb_device_error(0) == 0
+print("captured")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_rope_table_of_64_dimensions():
+    """alb_rope_table for head_dim 64, as the append reads it: angles by repeated fp32 products, each off by
+    half a step, so position p's angle i is off by (i + 1) u p and its cosine by that and the rounding."""
+    t = torch.empty(300, 32, 2, device="cuda")
+    A.check(L.alb_rope_table(t.data_ptr(), 300, 64, 1e6))
+    # theta_scale = powf(base, -2/64): its own rounding enters every product (one step at most)
+    tol = 300 * (3 * torch.arange(32)[None, :, None] + 4) * U + 2 * U
+    assert torch.all((t.double().cpu() - angles(300, 64).double().cpu()).abs() <= tol)
+
+
 def test_offsets_beyond_32_bits():
     """A pool of 2.2e9 elements whose used pages lie at its end."""
     page, hkv, dim = 64, 8, 128
