@@ -142,9 +142,10 @@ template <typename T> __device__ __noinline__ float lg_penalty_called(float f, u
     return lg_penalty<T>(f, c, RowRules{rep, freq, pres});
 }
 
-// T: the table's entries; TABLE: whether ids are counted or biased at all.
-template <typename T, bool TABLE>
-__global__ void __launch_bounds__(LG_THREADS, 3)
+// T: the table's entries; TABLE: whether ids are counted or biased at all; PER_SM:
+// CTAs an SM, 2 (64 registers a thread) or 3 (40, some spilled).
+template <typename T, bool TABLE, int PER_SM>
+__global__ void __launch_bounds__(LG_THREADS, PER_SM)
 k_logits(const __grid_constant__ LogitsArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     T * table = reinterpret_cast<T *>(smem);                            // [granules * 128]
@@ -420,16 +421,16 @@ k_logits(const __grid_constant__ LogitsArgs a) {
     }
 }
 
-template <typename T, bool TABLE>
+template <typename T, bool TABLE, int PER_SM>
 cudaError_t launch_logits(const LogitsArgs & a, int64_t rows, cudaStream_t st) {
     const size_t smem = (size_t)a.granules * LG_GRANULE * (TABLE ? sizeof(T) : 0) + (a.r.allow ? (size_t)a.granules * 16 : 0);
     const unsigned cluster = 1u << a.log_cluster;
     static std::atomic<bool> wide_clusters[64];   // per device: clusters of 16 are allowed
-    cudaError_t e = ensure_smem(k_logits<T, TABLE>, smem + LG_STATIC);   // the limit holds for both kinds together
+    cudaError_t e = ensure_smem(k_logits<T, TABLE, PER_SM>, smem + LG_STATIC);   // the limit holds for both kinds together
     int dev = 0;
     if (e == cudaSuccess && cluster > 8) e = cudaGetDevice(&dev);
     if (e == cudaSuccess && cluster > 8 && (dev >= 64 || !wide_clusters[dev].load(std::memory_order_acquire))) {
-        e = cudaFuncSetAttribute(k_logits<T, TABLE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        e = cudaFuncSetAttribute(k_logits<T, TABLE, PER_SM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess && dev < 64) wide_clusters[dev].store(true, std::memory_order_release);
     }
     if (e != cudaSuccess) return e;
@@ -446,7 +447,7 @@ cudaError_t launch_logits(const LogitsArgs & a, int64_t rows, cudaStream_t st) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, k_logits<T, TABLE>, a);
+    return cudaLaunchKernelEx(&cfg, k_logits<T, TABLE, PER_SM>, a);
 }
 
 }  // namespace
@@ -494,7 +495,13 @@ extern "C" int alb_logits_process(const float * logits, int64_t rows, int64_t n_
     a.granules = (int32_t)((granules + (1 << a.log_cluster) - 1) >> a.log_cluster);
     a.err = device_error_ptr();
     ALB_CUDA_TRY(a.err ? cudaSuccess : cudaErrorMemoryAllocation);
-    auto * f = !table ? launch_logits<uint16_t, false> : wide ? launch_logits<uint32_t, true> : launch_logits<uint16_t, true>;
+    // a call that two CTAs an SM hold runs with the registers that leaves (64 rows of 32003 with histories
+    // to 8192: 13.2 us against 18.4); where CTAs queue up a third one is worth more (256 rows of 151936:
+    // 85 us against 97)
+    const bool roomy = (rows << a.log_cluster) <= 2 * alb_sm_count();
+    auto * f = !table ? (roomy ? launch_logits<uint16_t, false, 2> : launch_logits<uint16_t, false, 3>)
+               : wide ? (roomy ? launch_logits<uint32_t, true, 2> : launch_logits<uint32_t, true, 3>)
+                      : (roomy ? launch_logits<uint16_t, true, 2> : launch_logits<uint16_t, true, 3>);
     ALB_CUDA_TRY(f(a, rows, (cudaStream_t)stream));
     return ALB_OK;
 }

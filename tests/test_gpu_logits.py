@@ -148,6 +148,7 @@ def same(x, kw, **more):
     (7, 1001, 100, 20, True), (4, 32003, 5000, 40, False), (3, 151936, 300, 0, False), (2, 151936, 9000, 300, True),
     (2, 262144, 700, 3, True), (1, 400001, 50, 2, True), (300, 257, 20, 2, True),
     (9, 185000, 40, 2, True), (9, 96000, 20000, 2, False), (1, 450000, 20000, 2, False),   # shared memory around its limits
+    (1000, 300, 20, 2, True), (120, 151936, 50, 3, True),   # many rows
 ])
 def test_rules(rows, vocab, hist, bias, mask):
     same(*case(np.random.default_rng(rows * vocab), rows, vocab, hist, bias, mask))
@@ -231,6 +232,16 @@ def test_padding_rows_are_left():
     wy, wn = plain(x, **kw)
     np.testing.assert_array_equal(y[[0, 2, 3]], wy[[0, 2, 3]])
     np.testing.assert_array_equal(n[[0, 2, 3]], wn[[0, 2, 3]])
+    # padding rows between others, many rows
+    x9, kw9 = case(np.random.default_rng(9), 900, 700, 30, 3, True)
+    pad = np.arange(900) % 7 == 2
+    kw9["lens"][pad] = -1
+    y, n = call(x9, **kw9)
+    assert (y[pad] == 7.5).all() and (n[pad] == -7).all()
+    kw9["lens"][pad] = 0
+    wy, wn = plain(x9, **kw9)
+    np.testing.assert_array_equal(y[~pad], wy[~pad])
+    np.testing.assert_array_equal(n[~pad], wn[~pad])
     kw["lens"][:] = -1
     y, n = call(x, **kw)
     assert (y == 7.5).all() and (n == -7).all()
@@ -320,9 +331,9 @@ def test_two_streams_and_a_replayed_graph():
 @pytest.mark.parametrize("vocab,hist", [(16000, 9000), (9000, 20000)])   # 16-bit and 32-bit counts
 def test_more_distinct_ids_than_a_cta_lists(vocab, hist):
     rng = np.random.default_rng(hist)
-    x, kw = case(rng, 160, vocab, hist, 20, True)
-    kw["history"] = rng.integers(0, vocab, (160, hist)).astype(np.int32)
-    kw["lens"][:] = rng.integers(0, hist + 1, 160)
+    x, kw = case(rng, 500, vocab, hist, 20, True)
+    kw["history"] = rng.integers(0, vocab, (500, hist)).astype(np.int32)
+    kw["lens"][:] = rng.integers(0, hist + 1, 500)
     kw["lens"][:3] = (hist, hist, 0)
     same(x, kw)
     same(x, kw, inplace=True)
