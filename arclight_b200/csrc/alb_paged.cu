@@ -55,6 +55,10 @@ template <> struct Vec<4> { using F = float4; };
 // its order.  The four sums are folded together (half the lanes keep two of them,
 // a quarter one): 6 exchanges instead of 20, and the eight lanes that end with a
 // head's sum find its scale, all four heads at once.
+// Bound by HBM on prompts: 8192 tokens of 32 / 8 heads move 373 MB in 68 us, 84 %
+// of the measured copy rate (one head a warp, with a division for the token: 136
+// us; blocks of four warps 73 us, of one 102 us).  A decode step is its launch
+// and four dependent loads, 2.6 us.
 constexpr int AP_HEADS = 4, AP_WARPS = 2;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(32 * AP_WARPS)
@@ -155,7 +159,10 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 
 // ---------------------------------------------------------------- attention
 // One pass over the cells with the running maximum and sum of a softmax, on the
-// tensor cores (mma m16n8k16, fp32 accumulators), everything in registers.
+// tensor cores (mma m16n8k16, fp32 accumulators), everything in registers.  Up to
+// 8 query heads share each byte, so the bytes bound the time and a fifth of the
+// rate of these warp-level products is needed; a tcgen05 tile of 128 rows would
+// hold the same 8 heads and want K and V in shared memory first.
 //
 // A unit is (row, K/V head, group of up to 8 query heads).  Its cells come in
 // tiles of 16 (D = 128) or 32, and all tiles of all units, each unit's led by a
@@ -183,6 +190,18 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // Exponents are base 2 and the running maximum is rounded up to a whole number,
 // so rescaling is exact; probabilities are scaled by 2^15 to stay clear of fp16's
 // subnormals (p >= 2^-24 of the largest keeps its leading part normal).
+//
+// Bound by HBM: 48 sequences of 8k to 32k cells (32 / 8 heads of 128) stream 4.2 GB
+// in 622 us, 6.75 TB/s; 37 ragged ones 110 us (bf16: with its three parts in one
+// product for up to four heads; two products 152 us).  A warp has a tile of K and V
+// (8 KB) in flight while it works on the one before, twelve warps an SM 96 KB; 16
+// warps at 128 registers spill (907 us), eight at 255 hold too little (676 us).  K
+// through the L1 cache, whose half lines the next load takes, is worth a tenth on
+// short calls.  Few rows are bound by the chain of dependent loads (lengths, page,
+// K and V; the join: what is unfinished, its pieces): one sequence of 640 cells
+// 8.3 us, of 32768 cells 32 us, 200 windows of single cells 22 us.  A unit's setup
+// weighs six tiles (0: 29 us for the windows and 122 for the ragged batch, 12:
+// 22.8 and 110).
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = 32 * PA_WARPS;
 constexpr int PA_CTAS_PER_SM = 3;        // what the registers allow (168 a thread)
@@ -723,7 +742,7 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
 #pragma unroll
                 for (int k = 0; k < N; ++k) acc[k] *= fix;
                 M = Mn;
-#pragma unroll 8
+#pragma unroll 4
                 for (int k = 0; PJ_PARTS * k + part < n; ++k) {
                     const float w = __shfl_sync(0xffffffffu, f, k);
                     float v[N];
