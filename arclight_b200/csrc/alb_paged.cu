@@ -167,16 +167,16 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // A unit is (row, K/V head, group of up to 8 query heads).  Its cells come in
 // tiles of 16 (D = 128) or 32, and all tiles of all units, each unit's led by a
 // few that stand for its setup, form one line that is cut into equal ranges, one
-// per CTA (k_paged_attn): uneven lengths and few rows load the SMs alike, and nothing depends on the lengths but device code.  In a CTA's
-// segment of a unit warp w takes every fourth tile; the warps join through
-// shared memory, and the pieces of a unit that a range's border cuts are joined
-// by k_paged_attn_join.
+// per CTA (k_paged_attn): uneven lengths and few rows load the SMs alike, and
+// nothing depends on the lengths but device code.  In a CTA's segment of a unit
+// warp w takes every fourth tile; the warps join through shared memory, and the
+// pieces of a unit that a range's border cuts are joined by k_paged_attn_join.
 //
 // Score product, S = Q K^T:  A (16 x 16) holds the 8 heads twice, rows 0-7 the
 // leading 11 bits of q and rows 8-15 the rest, so one instruction gives both
 // parts of S and c[0] + c[2], c[1] + c[3] their sum: q keeps 22 bits and more at
-// no extra instruction (bf16 caches: three parts of 8 bits, a second product for
-// the third).  Each row of q is scaled by a power of two first, so that its
+// no extra instruction.  bf16 caches need three parts of 8 bits: up to four heads
+// have them in rows 0-3, 4-7 and 8-11 (FOUR), more take a second product.  Each row of q is scaled by a power of two first, so that its
 // largest value has 10 bits before the point and no part underflows.
 // Value product, O = P V:  the accumulator layout of S is the A layout of P, so
 // the probabilities never leave their registers; they too are split in rows 0-7
