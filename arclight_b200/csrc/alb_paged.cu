@@ -192,8 +192,12 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // subnormals (p >= 2^-24 of the largest keeps its leading part normal).
 //
 // Bound by HBM: 48 sequences of 8k to 32k cells (32 / 8 heads of 128) stream 4.2 GB
-// in 622 us, 6.75 TB/s; 37 ragged ones 110 us (bf16: with its three parts in one
-// product for up to four heads; two products 152 us).  A warp has a tile of K and V
+// in 622 us, 6.75 TB/s; 37 ragged ones 110 us (bf16, its three parts in one
+// product for up to four heads).  bf16 with five to eight heads a group takes two
+// products and keeps the third parts of q in shared memory: 64 sequences of 4k to
+// 8k cells 5.3 TB/s (4.3 with all parts in registers, which spill), where four
+// heads stream 6.6.  More than eight heads read K and V again for each eight,
+// mostly from the L2 cache.  A warp has a tile of K and V
 // (8 KB) in flight while it works on the one before, twelve warps an SM 96 KB; 16
 // warps at 128 registers spill (907 us), eight at 255 hold too little (676 us).  K
 // through the L1 cache, whose half lines the next load takes, is worth a tenth on
@@ -333,6 +337,9 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
     constexpr int PITCH = D + 4;
     __shared__ __align__(16) float so[PA_WARPS][8][PITCH];
     __shared__ float sm[PA_WARPS][8], sl[PA_WARPS][8];
+    // the third parts of q for products with bf16 of more than four heads, a lane's own (registers would spill)
+    constexpr bool THIRD = BF16 && !FOUR;
+    __shared__ __align__(16) uint4 sq[THIRD ? PA_WARPS : 1][THIRD ? KL : 1][32];
     __shared__ int64_t warp_sum[PA_WARPS];
     __shared__ int32_t at_row, at_unit, at_tile;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -479,7 +486,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         uint32_t off = offset_of(page, pos);
         load_k(off);
         load_v(off);
-        uint32_t qh[KL][4], qm[KL][4], ql[BF16 && !FOUR ? KL : 1][4];
+        uint32_t qh[KL][4], qm[KL][4];
         float c;
         {
 #pragma unroll
@@ -496,20 +503,17 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             c = e > 0 ? a.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23)
                       : a.scale_log2 * (1.0f / up);
 #pragma unroll
-            for (int i = 0; i < KL; ++i)
+            for (int i = 0; i < KL; ++i) {
+                uint32_t l[4];
 #pragma unroll
                 for (int e2 = 0; e2 < 4; ++e2) {
-                    uint32_t h, m, l;
-                    pa_split<BF16>(qv[i][2 * e2] * up, qv[i][2 * e2 + 1] * up, h, m, l);
-                    if (FOUR) {   // rows 0-3, 4-7, 8-11 of A
-                        qh[i][e2] = g < 4 ? h : m;
-                        qm[i][e2] = g < 4 ? l : 0u;
-                    } else {
-                        qh[i][e2] = h;
-                        qm[i][e2] = m;
-                        if (BF16) ql[i][e2] = l;
-                    }
+                    uint32_t h, m;
+                    pa_split<BF16>(qv[i][2 * e2] * up, qv[i][2 * e2 + 1] * up, h, m, l[e2]);
+                    qh[i][e2] = FOUR && g >= 4 ? m : h;                      // FOUR: rows 0-3, 4-7, 8-11 of A
+                    qm[i][e2] = !FOUR ? m : g < 4 ? l[e2] : 0u;
                 }
+                if (THIRD) sq[warp][i][lane] = make_uint4(l[0], l[1], l[2], l[3]);
+            }
         }
 
         float o[VH][8][2], m = -INFINITY, l = 0.0f;
@@ -532,9 +536,10 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                         if (k == 0) pa_mma0<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], w.x, w.y);
                         else        pa_mma<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], w.x, w.y);
                         pa_mma<BF16>(s[u], qh[k][2], qm[k][2], qh[k][3], qm[k][3], w.z, w.w);
-                        if (BF16 && !FOUR) {
-                            pa_mma<BF16>(s[u], ql[k][0], 0u, ql[k][1], 0u, w.x, w.y);
-                            pa_mma<BF16>(s[u], ql[k][2], 0u, ql[k][3], 0u, w.z, w.w);
+                        if (THIRD) {
+                            const uint4 l = sq[warp][k][lane];
+                            pa_mma<BF16>(s[u], l.x, 0u, l.y, 0u, w.x, w.y);
+                            pa_mma<BF16>(s[u], l.z, 0u, l.w, 0u, w.z, w.w);
                         }
                     }
                 }
@@ -591,7 +596,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                         const uint32_t b0 = __byte_perm(word(0), word(1), sel), b1 = __byte_perm(word(2), word(3), sel);
                         if (b == 0) pa_mma0<BF16>(r, ph[b][0], pm[b][0], ph[b][1], pm[b][1], b0, b1);
                         else        pa_mma<BF16>(r, ph[b][0], pm[b][0], ph[b][1], pm[b][1], b0, b1);
-                        if (BF16 && !FOUR) pa_mma<BF16>(r, pl[b][0], 0u, pl[b][1], 0u, b0, b1);
+                        if (THIRD) pa_mma<BF16>(r, pl[b][0], 0u, pl[b][1], 0u, b0, b1);
                     }
                     o[h][j][0] = fmaf(o[h][j][0], fix, r[0] + r[2]);
                     o[h][j][1] = fmaf(o[h][j][1], fix, r[1] + r[3]);
