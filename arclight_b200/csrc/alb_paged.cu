@@ -164,7 +164,8 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // rate of these warp-level products is needed; a tcgen05 tile of 128 rows would
 // hold the same 8 heads and want K and V in shared memory first.
 //
-// A unit is (row, K/V head, group of up to 8 query heads).  Its cells come in
+// A unit is (row, K/V head, group of up to 8 query heads; 16 where more share
+// the K/V head).  Its cells come in
 // tiles of 16 (D = 128) or 32, and all tiles of all units, each unit's led by a
 // few that stand for its setup, form one line that is cut into equal ranges, one
 // per CTA (k_paged_attn): uneven lengths and few rows load the SMs alike, and
@@ -208,10 +209,11 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // 22.8 and 110).
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = 32 * PA_WARPS;
-constexpr int PA_CTAS_PER_SM = 3;        // what the registers allow (168 a thread)
+// CTAs per SM: what the registers allow (168 a thread for units of 8 heads, 255 for units of 16)
+template <int R> constexpr int PA_CTAS_PER_SM = R == 1 ? 3 : 2;
 // Cells of a tile: 16 per product step, 8 KB of K and V in a warp's registers either way.
 template <int D> constexpr int PA_TILE = 16 * 128 / D;
-constexpr int PA_MAX_CTAS = 1024;
+constexpr int PA_MAX_CTAS = 1024;        // of units of 8 heads; of 16: half as many
 constexpr int PA_MIN_TILES = 4;          // a CTA's range is at least a tile per warp
 constexpr int PA_SETUP = 6;              // what a unit costs beside its tiles, in tiles
 constexpr float PA_SHIFT = 15.0f;
@@ -222,9 +224,10 @@ constexpr float PA_SHIFT = 15.0f;
 // The pieces' maxima and sums by head, [0] the CTA's head, [1] its tail.
 struct PaMeta {
     int32_t tail_row[PA_MAX_CTAS], tail_unit[PA_MAX_CTAS], head_ends[PA_MAX_CTAS];
-    float m[2][8][PA_MAX_CTAS], l[2][8][PA_MAX_CTAS];
+    float m[2][16][PA_MAX_CTAS], l[2][16][PA_MAX_CTAS];
 };
-template <int D> struct PaPiece { float o[8][D]; };
+// A piece's sums: [8 R heads][D], head of CTA c at place 2 c, its tail at 2 c + 1.
+template <int D, int R> __host__ __device__ constexpr size_t pa_piece_floats() { return (size_t)8 * R * D; }
 
 struct PaArgs {
     const float * q;
@@ -234,7 +237,7 @@ struct PaArgs {
     int32_t Hq, G, groups, window;
     float scale_log2;
     PaMeta * meta;
-    void * pieces;
+    float * pieces;
     float * out, * lse;
     int * err;
 };
@@ -329,17 +332,22 @@ __device__ __forceinline__ void pa_split(float x, float y, uint32_t & hi, uint32
     }
 }
 
-template <int D, bool BF16, bool FOUR>
-__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM)
+// R: heads of a unit / 8.  R = 1 has two parts of its 8 heads in a product's 16
+// rows (FOUR: three parts of up to 4), R = 2 a part of 16 heads, product by product.
+template <int D, bool BF16, bool FOUR, int R>
+__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM<R>)
 k_paged_attn(const __grid_constant__ PaArgs a) {
     constexpr int KL = D / 32, VH = D / 64;       // 16-byte loads of K per cell and lane; 64-value halves of V
     constexpr int TILE = PA_TILE<D>, SUB = TILE / 16;
     constexpr int PITCH = D + 4;
-    __shared__ __align__(16) float so[PA_WARPS][8][PITCH];
-    __shared__ float sm[PA_WARPS][8], sl[PA_WARPS][8];
-    // the third parts of q for products with bf16 of more than four heads, a lane's own (registers would spill)
-    constexpr bool THIRD = BF16 && !FOUR;
-    __shared__ __align__(16) uint4 sq[THIRD ? PA_WARPS : 1][THIRD ? KL : 1][32];
+    // Parts of q that do not stay in registers (they would spill), a lane's own: the third for R = 1
+    // with bf16 of more than four heads, all but the first for R = 2.
+    constexpr int PARTS = BF16 ? 3 : 2, REST = R == 2 ? 2 * (PARTS - 1) : BF16 && !FOUR ? 1 : 0;
+    constexpr size_t SO = (size_t)PA_WARPS * 8 * R * PITCH * 4, SQ = (size_t)PA_WARPS * REST * KL * 512;
+    __shared__ __align__(16) uint8_t shared[(R == 1 ? SO + SQ : SO > SQ ? SO : SQ)];   // R = 2: one after the other
+    float (* so)[8 * R][PITCH] = reinterpret_cast<float (*)[8 * R][PITCH]>(shared);
+    uint4 (* sq)[REST ? REST : 1][KL][32] = reinterpret_cast<uint4 (*)[REST ? REST : 1][KL][32]>(shared + (R == 1 ? SO : 0));
+    __shared__ float sm[PA_WARPS][8 * R], sl[PA_WARPS][8 * R];
     __shared__ int64_t warp_sum[PA_WARPS];
     __shared__ int32_t at_row, at_unit, at_tile;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -420,8 +428,8 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         const int32_t n = begins ? tile + take : take;
         lo += max(tile, 0) * TILE;
         const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
-        const int heads = min(8, a.G - 8 * grp);
-        const int32_t head0 = kvh * a.G + 8 * grp;
+        const int heads = min(8 * R, a.G - 8 * R * grp);
+        const int32_t head0 = kvh * a.G + 8 * R * grp;
         const int gh = FOUR ? g & 3 : g;   // this lane's head
         const int32_t * table = a.kv.table + (int64_t)seq * a.kv.table_stride;
         const uint8_t * kb = reinterpret_cast<const uint8_t *>(a.kv.k + (int64_t)kvh * a.kv.head_stride + 8 * t);
@@ -443,18 +451,18 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         int32_t page = page_at(warp, pos);
         int32_t page2 = page_at(warp + PA_WARPS, pos2);
 
-        // q of head g: its values 32 i + 8 t .. + 7 are k steps 2 i and 2 i + 1 of this lane
-        float qv[KL][8];
-        float top = 0.0f;
-        {
-            const float * qr = a.q + ((int64_t)row * a.Hq + head0 + gh) * D + 8 * t;
+        // q of head g (and g + 8): its values 32 i + 8 t .. + 7 are k steps 2 i and 2 i + 1 of this lane
+        float qv[R][KL][8];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float * qr = a.q + ((int64_t)row * a.Hq + head0 + gh + 8 * r) * D + 8 * t;
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) qv[i][e] = 0.0f;
-                if (gh < heads) {
-                    *reinterpret_cast<float4 *>(qv[i]) = *reinterpret_cast<const float4 *>(qr + 32 * i);
-                    *reinterpret_cast<float4 *>(qv[i] + 4) = *reinterpret_cast<const float4 *>(qr + 32 * i + 4);
+                for (int e = 0; e < 8; ++e) qv[r][i][e] = 0.0f;
+                if (gh + 8 * r < heads) {
+                    *reinterpret_cast<float4 *>(qv[r][i]) = *reinterpret_cast<const float4 *>(qr + 32 * i);
+                    *reinterpret_cast<float4 *>(qv[r][i] + 4) = *reinterpret_cast<const float4 *>(qr + 32 * i + 4);
                 }
             }
         }
@@ -486,13 +494,17 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
         uint32_t off = offset_of(page, pos);
         load_k(off);
         load_v(off);
-        uint32_t qh[KL][4], qm[KL][4];
-        float c;
-        {
+        // A's rows 0-7 and 8-15 of the first product: R = 1 the first and second parts of its heads (FOUR:
+        // first, second, third and nothing in fours), R = 2 the first parts of heads 0-7 and 8-15
+        uint32_t qa[KL][4], qb[KL][4];
+        float c[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < KL; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(qv[i][e]));
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(qv[r][i][e]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // 2^e with top 2^e in [2^9, 2^10); nothing to scale for 0 and what is not finite
@@ -500,31 +512,44 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             int e = ex == 255 || top == 0.0f ? 0 : 127 + 9 - max(ex, 1);
             e = min(e, 126);
             const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-            c = e > 0 ? a.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23)
-                      : a.scale_log2 * (1.0f / up);
+            c[r] = e > 0 ? a.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) : a.scale_log2 * (1.0f / up);
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
-                uint32_t l[4];
+                uint32_t h[4], m[4], l[4];
+#pragma unroll
+                for (int e2 = 0; e2 < 4; ++e2)
+                    pa_split<BF16>(qv[r][i][2 * e2] * up, qv[r][i][2 * e2 + 1] * up, h[e2], m[e2], l[e2]);
 #pragma unroll
                 for (int e2 = 0; e2 < 4; ++e2) {
-                    uint32_t h, m;
-                    pa_split<BF16>(qv[i][2 * e2] * up, qv[i][2 * e2 + 1] * up, h, m, l[e2]);
-                    qh[i][e2] = FOUR && g >= 4 ? m : h;                      // FOUR: rows 0-3, 4-7, 8-11 of A
-                    qm[i][e2] = !FOUR ? m : g < 4 ? l[e2] : 0u;
+                    if (R == 2) {
+                        if (r == 0) qa[i][e2] = h[e2];
+                        else        qb[i][e2] = h[e2];
+                    } else {
+                        qa[i][e2] = FOUR && g >= 4 ? m[e2] : h[e2];
+                        qb[i][e2] = !FOUR ? m[e2] : g < 4 ? l[e2] : 0u;
+                    }
                 }
-                if (THIRD) sq[warp][i][lane] = make_uint4(l[0], l[1], l[2], l[3]);
+                if (R == 2) {
+                    sq[warp][r][i][lane] = make_uint4(m[0], m[1], m[2], m[3]);
+                    if (BF16) sq[warp][2 + r][i][lane] = make_uint4(l[0], l[1], l[2], l[3]);
+                } else if (REST) {
+                    sq[warp][0][i][lane] = make_uint4(l[0], l[1], l[2], l[3]);
+                }
             }
         }
 
-        float o[VH][8][2], m = -INFINITY, l = 0.0f;
+        float o[VH][8][2 * R], m[R], l[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) { m[r] = -INFINITY; l[r] = 0.0f; }
 #pragma unroll
         for (int h = 0; h < VH; ++h)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[h][j][0] = o[h][j][1] = 0.0f;
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int p = 0; p < 2 * R; ++p) o[h][j][p] = 0.0f;
 
         for (int32_t i = warp; i < n; i += PA_WARPS) {
-            float x[SUB][4];   // scores of cells 16 b + 2t, 2t + 1, 2t + 8, 2t + 9
-            float top = -INFINITY;
+            float x[R][SUB][4];   // scores of cells 16 b + 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
             for (int b = 0; b < SUB; ++b) {
                 float s[2][4];
@@ -533,54 +558,72 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
                     for (int k = 0; k < KL; ++k) {
                         const uint4 & w = K[b][u][k];
-                        if (k == 0) pa_mma0<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], w.x, w.y);
-                        else        pa_mma<BF16>(s[u], qh[k][0], qm[k][0], qh[k][1], qm[k][1], w.x, w.y);
-                        pa_mma<BF16>(s[u], qh[k][2], qm[k][2], qh[k][3], qm[k][3], w.z, w.w);
-                        if (THIRD) {
-                            const uint4 l = sq[warp][k][lane];
-                            pa_mma<BF16>(s[u], l.x, 0u, l.y, 0u, w.x, w.y);
-                            pa_mma<BF16>(s[u], l.z, 0u, l.w, 0u, w.z, w.w);
+                        if (k == 0) pa_mma0<BF16>(s[u], qa[k][0], qb[k][0], qa[k][1], qb[k][1], w.x, w.y);
+                        else        pa_mma<BF16>(s[u], qa[k][0], qb[k][0], qa[k][1], qb[k][1], w.x, w.y);
+                        pa_mma<BF16>(s[u], qa[k][2], qb[k][2], qa[k][3], qb[k][3], w.z, w.w);
+                        if (R == 2) {
+#pragma unroll
+                            for (int p = 0; p < PARTS - 1; ++p) {
+                                const uint4 y = sq[warp][2 * p][k][lane], z = sq[warp][2 * p + 1][k][lane];
+                                pa_mma<BF16>(s[u], y.x, z.x, y.y, z.y, w.x, w.y);
+                                pa_mma<BF16>(s[u], y.z, z.z, y.w, z.w, w.z, w.w);
+                            }
+                        } else if (REST) {
+                            const uint4 y = sq[warp][0][k][lane];
+                            pa_mma<BF16>(s[u], y.x, 0u, y.y, 0u, w.x, w.y);
+                            pa_mma<BF16>(s[u], y.z, 0u, y.w, 0u, w.z, w.w);
                         }
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) x[b][u] = s[u >> 1][u & 1] + s[u >> 1][2 + (u & 1)];
+                for (int u = 0; u < 4; ++u) {
+                    if (R == 2) {
+                        x[0][b][u] = s[u >> 1][u & 1];
+                        x[R - 1][b][u] = s[u >> 1][2 + (u & 1)];
+                    } else {
+                        x[0][b][u] = s[u >> 1][u & 1] + s[u >> 1][2 + (u & 1)];
+                    }
+                }
             }
             // the next tile's K comes while this tile's softmax and values are worked on
             off = offset_of(page2, pos2);
             load_k(off);
             page2 = page_at(i + 2 * PA_WARPS, pos2);
 
+            float fix[R];
+            uint32_t part[PARTS][R][SUB][2];   // of the probabilities, by weight
 #pragma unroll
-            for (int b = 0; b < SUB; ++b)
+            for (int r = 0; r < R; ++r) {
+                float top = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (FOUR) x[b][u] += __shfl_xor_sync(0xffffffffu, x[b][u], 16);   // the parts in rows g and g + 4
-                    top = fmaxf(top, ok[b][u] ? __fmul_rn(x[b][u], c) : -INFINITY);
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float mn = fmaxf(m, ceilf(top));
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            const float fix = pa_ex2(m - base);
-            m = mn;
-            // one rounding from the score on, as long as the maximum of the rounded products is
-            // within 2^-8 of the exact ones' (2^16 has steps of 2^-7); the rounded products beyond
-            const bool big = !(fabsf(base) < 65536.0f);
-            l *= fix;
-            uint32_t ph[SUB][2], pm[SUB][2], pl[SUB][2];
+                for (int b = 0; b < SUB; ++b)
 #pragma unroll
-            for (int b = 0; b < SUB; ++b) {
+                    for (int u = 0; u < 4; ++u) {
+                        if (FOUR) x[r][b][u] += __shfl_xor_sync(0xffffffffu, x[r][b][u], 16);   // the parts in rows g and g + 4
+                        top = fmaxf(top, ok[b][u] ? __fmul_rn(x[r][b][u], c[r]) : -INFINITY);
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float mn = fmaxf(m[r], ceilf(top));
+                const float base = mn == -INFINITY ? 0.0f : mn;
+                fix[r] = pa_ex2(m[r] - base);
+                m[r] = mn;
+                // one rounding from the score on, as long as the maximum of the rounded products is
+                // within 2^-8 of the exact ones' (2^16 has steps of 2^-7); the rounded products beyond
+                const bool big = !(fabsf(base) < 65536.0f);
+                l[r] *= fix[r];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    x[b][u] = !ok[b][u] ? 0.0f : pa_ex2(big ? __fmul_rn(x[b][u], c) - base + PA_SHIFT : fmaf(x[b][u], c, PA_SHIFT - base));
-                l += (x[b][0] + x[b][1]) + (x[b][2] + x[b][3]);
+                for (int b = 0; b < SUB; ++b) {
+                    float (& y)[4] = x[r][b];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    pa_split<BF16>(x[b][2 * u], x[b][2 * u + 1], ph[b][u], pm[b][u], pl[b][u]);
-                    if (FOUR) {
-                        ph[b][u] = g < 4 ? ph[b][u] : pm[b][u];
-                        pm[b][u] = g < 4 ? pl[b][u] : 0u;
+                    for (int u = 0; u < 4; ++u)
+                        y[u] = !ok[b][u] ? 0.0f : pa_ex2(big ? __fmul_rn(y[u], c[r]) - base + PA_SHIFT : fmaf(y[u], c[r], PA_SHIFT - base));
+                    l[r] += (y[0] + y[1]) + (y[2] + y[3]);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        uint32_t last;
+                        pa_split<BF16>(y[2 * u], y[2 * u + 1], part[0][r][b][u], part[1][r][b][u], last);
+                        if (BF16) part[PARTS - 1][r][b][u] = last;
                     }
                 }
             }
@@ -594,12 +637,30 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                     for (int b = 0; b < SUB; ++b) {
                         auto word = [&](int u) { return reinterpret_cast<const uint32_t *>(&V[b][u][h])[j >> 1]; };
                         const uint32_t b0 = __byte_perm(word(0), word(1), sel), b1 = __byte_perm(word(2), word(3), sel);
-                        if (b == 0) pa_mma0<BF16>(r, ph[b][0], pm[b][0], ph[b][1], pm[b][1], b0, b1);
-                        else        pa_mma<BF16>(r, ph[b][0], pm[b][0], ph[b][1], pm[b][1], b0, b1);
-                        if (THIRD) pa_mma<BF16>(r, pl[b][0], 0u, pl[b][1], 0u, b0, b1);
+                        if (R == 2) {
+#pragma unroll
+                            for (int p = 0; p < PARTS; ++p) {
+                                uint32_t (& y)[SUB][2] = part[p][0], (& z)[SUB][2] = part[p][R - 1];
+                                if (b == 0 && p == 0) pa_mma0<BF16>(r, y[b][0], z[b][0], y[b][1], z[b][1], b0, b1);
+                                else                  pa_mma<BF16>(r, y[b][0], z[b][0], y[b][1], z[b][1], b0, b1);
+                            }
+                        } else {
+                            const uint32_t y0 = FOUR && g >= 4 ? part[1][0][b][0] : part[0][0][b][0];
+                            const uint32_t y1 = FOUR && g >= 4 ? part[1][0][b][1] : part[0][0][b][1];
+                            const uint32_t z0 = !FOUR ? part[1][0][b][0] : g < 4 ? part[PARTS - 1][0][b][0] : 0u;
+                            const uint32_t z1 = !FOUR ? part[1][0][b][1] : g < 4 ? part[PARTS - 1][0][b][1] : 0u;
+                            if (b == 0) pa_mma0<BF16>(r, y0, z0, y1, z1, b0, b1);
+                            else        pa_mma<BF16>(r, y0, z0, y1, z1, b0, b1);
+                            if (REST) pa_mma<BF16>(r, part[PARTS - 1][0][b][0], 0u, part[PARTS - 1][0][b][1], 0u, b0, b1);
+                        }
                     }
-                    o[h][j][0] = fmaf(o[h][j][0], fix, r[0] + r[2]);
-                    o[h][j][1] = fmaf(o[h][j][1], fix, r[1] + r[3]);
+                    if (R == 2) {
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) o[h][j][p & (2 * R - 1)] = fmaf(o[h][j][p & (2 * R - 1)], fix[(p >> 1) & (R - 1)], r[p]);
+                    } else {
+                        o[h][j][0] = fmaf(o[h][j][0], fix[0], r[0] + r[2]);
+                        o[h][j][1] = fmaf(o[h][j][1], fix[0], r[1] + r[3]);
+                    }
                 }
             }
             load_v(off);
@@ -614,22 +675,26 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                     for (int p = 0; p < 2; ++p) o[h][j][p] += __shfl_xor_sync(0xffffffffu, o[h][j][p], 16);
         }
 
-        // ---- join the warps: thread (head, part) adds its D / 16 values
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) { sm[warp][g] = m; sl[warp][g] = l; }
+        // ---- join the warps: thread (head, part) adds its values
+        if (R == 2) __syncthreads();   // the shared parts of q make room for the sums
 #pragma unroll
-        for (int h = 0; h < VH; ++h)
+        for (int r = 0; r < R; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (t == 0) { sm[warp][g + 8 * r] = m[r]; sl[warp][g + 8 * r] = l[r]; }
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
+            for (int h = 0; h < VH; ++h)
 #pragma unroll
-                for (int j = 0; j < 8; j += 4)
-                    *reinterpret_cast<float4 *>(&so[warp][g][64 * h + 16 * t + 8 * p + j]) =
-                        make_float4(o[h][j][p], o[h][j + 1][p], o[h][j + 2][p], o[h][j + 3][p]);
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int j = 0; j < 8; j += 4)
+                        *reinterpret_cast<float4 *>(&so[warp][g + 8 * r][64 * h + 16 * t + 8 * p + j]) =
+                            make_float4(o[h][j][2 * r + p], o[h][j + 1][2 * r + p], o[h][j + 2][2 * r + p], o[h][j + 3][2 * r + p]);
+        }
         __syncthreads();
         {
-            constexpr int N = D / 16;
-            const int h = tid >> 4, d = (tid & 15) * N;
+            constexpr int N = D * R / 16, PER = 16 / R;   // values of a thread, threads of a head
+            const int h = tid / PER, d = tid % PER * N;
             float M = sm[0][h];
 #pragma unroll
             for (int w = 1; w < PA_WARPS; ++w) M = fmaxf(M, sm[w][h]);
@@ -658,15 +723,15 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
                     for (int e = 0; e < N; e += 4)
                         *reinterpret_cast<float4 *>(dst + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-                    if (a.lse && (tid & 15) == 0)
+                    if (a.lse && d == 0)
                         a.lse[(int64_t)row * a.Hq + head0 + h] =
                             Ls != 0.0f ? fmaf(M, 0.693147181f, logf(Ls * 0x1p-15f)) : -INFINITY;
                 } else {
-                    PaPiece<D> * piece = static_cast<PaPiece<D> *>(a.pieces) + 2 * cta + (begins ? 1 : 0);
+                    float * piece = a.pieces + (2 * cta + (begins ? 1 : 0)) * pa_piece_floats<D, R>() + h * D + d;
 #pragma unroll
                     for (int e = 0; e < N; e += 4)
-                        *reinterpret_cast<float4 *>(&piece->o[h][d + e]) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-                    if ((tid & 15) == 0) { a.meta->m[begins][h][cta] = M; a.meta->l[begins][h][cta] = Ls; }
+                        *reinterpret_cast<float4 *>(piece + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+                    if (d == 0) { a.meta->m[begins][h][cta] = M; a.meta->l[begins][h][cta] = Ls; }
                 }
             }
             if (!begins) head_ends = ends;
@@ -694,7 +759,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 // pieces a warp and round; the pieces' maxima are whole numbers, so rescaling is exact
 // whatever the order.
 constexpr int PJ_HEADS = 2, PJ_PARTS = 4, PJ_THREADS = 32 * PJ_HEADS * PJ_PARTS;
-template <int D>
+template <int D, int R>
 __global__ void __launch_bounds__(PJ_THREADS)
 k_paged_attn_join(const __grid_constant__ PaArgs a) {
     constexpr int N = D / 32;
@@ -704,9 +769,8 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
     __shared__ __align__(16) float so[PJ_HEADS][PJ_PARTS][D];
     __shared__ float sm[PJ_HEADS][PJ_PARTS], sl[PJ_HEADS][PJ_PARTS];
     alb_pdl_wait();
-    const PaPiece<D> * pieces = static_cast<const PaPiece<D> *>(a.pieces);
-    // piece i: the tail of this CTA, then the head of the i-th CTA behind it
-    auto piece = [&](int i) { return pieces + 2 * (cta + i) + (i == 0 ? 1 : 0); };
+    // piece i's sums: the tail of this CTA, then the head of the i-th CTA behind it
+    auto piece = [&](int i) { return a.pieces + (2 * (cta + i) + (i == 0 ? 1 : 0)) * pa_piece_floats<D, R>(); };
     // lane l looks after pieces PARTS l .. of a round for where the unit ends, after PARTS l + part for its weight
     int last;                 // place of the first end among this lane's, or PARTS
     float m, l;
@@ -730,7 +794,7 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
     const int32_t row = a.meta->tail_row[cta], unit = a.meta->tail_unit[cta];
     look(0);
     const int32_t kvh = unit / a.groups, grp = unit - kvh * a.groups;
-    const int heads = min(8, a.G - 8 * grp);
+    const int heads = min(8 * R, a.G - 8 * R * grp);
     if (row >= 0 && PJ_HEADS * (int)blockIdx.y < heads) {   // uniform over the block
         float M = -INFINITY, L = 0.0f, acc[N];
 #pragma unroll
@@ -751,7 +815,7 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
                 for (int k = 0; PJ_PARTS * k + part < n; ++k) {
                     const float w = __shfl_sync(0xffffffffu, f, k);
                     float v[N];
-                    *reinterpret_cast<F *>(v) = *reinterpret_cast<const F *>(&piece(i0 + PJ_PARTS * k + part)->o[h][N * lane]);
+                    *reinterpret_cast<F *>(v) = *reinterpret_cast<const F *>(piece(i0 + PJ_PARTS * k + part) + h * D + N * lane);
 #pragma unroll
                     for (int j = 0; j < N; ++j) acc[j] = fmaf(v[j], w, acc[j]);
                 }
@@ -780,7 +844,7 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) acc[e] = fmaf(v[e], f, acc[e]);
             }
-            const int64_t head = (int64_t)row * a.Hq + kvh * a.G + 8 * grp + h;
+            const int64_t head = (int64_t)row * a.Hq + kvh * a.G + 8 * R * grp + h;
 #pragma unroll
             for (int e = 0; e < N; ++e) acc[e] = L != 0.0f ? acc[e] / L : 0.0f;
             *reinterpret_cast<F *>(a.out + head * D + N * lane) = *reinterpret_cast<F *>(acc);
@@ -869,18 +933,23 @@ cudaError_t launch_append(const float * qkv, int64_t qkv_stride, int64_t T, int 
                       qkv, qkv_stride, Hq, qn, kn, eps, rope, max_pos, positions, seqs, kv, q_out, err);
 }
 
-size_t attn_ws_bytes(int D) {
-    return sizeof(PaMeta) + 2 * PA_MAX_CTAS * (D == 128 ? sizeof(PaPiece<128>) : sizeof(PaPiece<64>));
+size_t attn_ws_bytes(int D) { return sizeof(PaMeta) + 2 * PA_MAX_CTAS * 8 * (size_t)D * sizeof(float); }
+
+template <int D, bool BF16, bool FOUR, int R>
+cudaError_t launch_attn_r(PaArgs a, cudaStream_t st) {
+    a.groups = (a.G + 8 * R - 1) / (8 * R);
+    const int ctas = min(PA_MAX_CTAS / R, PA_CTAS_PER_SM<R> * alb_sm_count());
+    cudaError_t e = alb_launch(k_paged_attn<D, BF16, FOUR, R>, dim3((unsigned)ctas), dim3(PA_THREADS), 0, st, true, a);
+    if (e != cudaSuccess) return e;
+    const unsigned parts = (unsigned)(min(a.G, 8 * R) + PJ_HEADS - 1) / PJ_HEADS;
+    return alb_launch(k_paged_attn_join<D, R>, dim3((unsigned)ctas, parts), dim3(PJ_THREADS), 0, st, true, a);
 }
 
 template <int D, bool BF16>
 cudaError_t launch_attn(const PaArgs & a, cudaStream_t st) {
-    const int ctas = min(PA_MAX_CTAS, PA_CTAS_PER_SM * alb_sm_count());
-    auto * f = BF16 && a.G <= 4 ? k_paged_attn<D, BF16, BF16> : k_paged_attn<D, BF16, false>;
-    cudaError_t e = alb_launch(f, dim3((unsigned)ctas), dim3(PA_THREADS), 0, st, true, a);
-    if (e != cudaSuccess) return e;
-    const unsigned parts = (unsigned)(min(a.G, 8) + PJ_HEADS - 1) / PJ_HEADS;
-    return alb_launch(k_paged_attn_join<D>, dim3((unsigned)ctas, parts), dim3(PJ_THREADS), 0, st, true, a);
+    // more than 8 heads a group: units of 16, which read K and V once
+    if (a.G > 8) return launch_attn_r<D, BF16, false, 2>(a, st);
+    return BF16 && a.G <= 4 ? launch_attn_r<D, BF16, BF16, 1>(a, st) : launch_attn_r<D, BF16, false, 1>(a, st);
 }
 
 }  // namespace
@@ -924,9 +993,9 @@ extern "C" int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, c
     ALB_CHECK_ARG((((uintptr_t)lengths | (uintptr_t)seqs | (uintptr_t)lse) & 3) == 0);
     PaArgs a = {};
     a.q = q; a.kv = v; a.seqs = seqs; a.lengths = lengths; a.n_rows = n_rows; a.Hq = n_head; a.G = n_head / v.Hkv;
-    a.groups = (a.G + 7) / 8; a.window = window; a.scale_log2 = scale * 1.44269504f; a.out = out; a.lse = lse;
+    a.window = window; a.scale_log2 = scale * 1.44269504f; a.out = out; a.lse = lse;
     a.meta = static_cast<PaMeta *>(workspace);
-    a.pieces = static_cast<uint8_t *>(workspace) + sizeof(PaMeta);
+    a.pieces = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + sizeof(PaMeta));
     a.err = device_error_ptr();
     ALB_CUDA_TRY(a.err ? cudaSuccess : cudaErrorMemoryAllocation);
     auto * f = kv->head_dim == 128 ? (kv->type == ALB_KV_BF16 ? launch_attn<128, true> : launch_attn<128, false>)
