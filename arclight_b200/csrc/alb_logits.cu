@@ -13,7 +13,7 @@
 // mask, maximum.  The CTAs' maxima go to CTA 0's shared memory.
 //
 // Bound by instruction issue and the chain of dependent steps, not by HBM: 256
-// rows of 151936 with histories to 4096 and masks take 85 us (314 MB, 3.7 TB/s;
+// rows of 151936 with histories to 4096 and masks take 83 us (314 MB, 3.8 TB/s;
 // about 60 issued instructions per group of four tokens and 80 per id and CTA that
 // reads it), 48 rows with biases and masks 20 us, 64 rows of 32003 with histories
 // to 8192 13 us, one row 4.8 us.  Other shapes that were measured on the first of
@@ -60,7 +60,8 @@ struct LogitsArgs {
     int * err;
 };
 
-__device__ __forceinline__ void lg_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+// (relaxed: all that lies before it is the barrier's own initialisation, which has its fence)
+__device__ __forceinline__ void lg_cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void lg_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t lg_remote(const void * local, uint32_t rank) {
     uint32_t a;
@@ -507,7 +508,7 @@ extern "C" int alb_logits_process(const float * logits, int64_t rows, int64_t n_
     ALB_CUDA_TRY(a.err ? cudaSuccess : cudaErrorMemoryAllocation);
     // a call that two CTAs an SM hold runs with the registers that leaves (64 rows of 32003 with histories
     // to 8192: 13.2 us against 18.4); where CTAs queue up a third one is worth more (256 rows of 151936:
-    // 85 us against 97)
+    // 83 us against 97)
     const bool roomy = (rows << a.log_cluster) <= 2 * alb_sm_count();
     auto * f = !table ? (roomy ? launch_logits<uint16_t, false, 2> : launch_logits<uint16_t, false, 3>)
                : wide ? (roomy ? launch_logits<uint32_t, true, 2> : launch_logits<uint32_t, true, 3>)
