@@ -252,21 +252,23 @@ ALB_API int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, int
  * seqs[r] (device int32; seqs NULL: sequence r; window 0: no limit), its own token
  * included when that is already in the cache:
  *   out[r][h] = sum_j exp(s_j - m) V_j / sum_j exp(s_j - m),  s_j = scale q . K_j,
- * m the largest s_j and h / (n_head / n_head_kv) the K/V head (any whole ratio).
- * lse [n_rows][n_head] (nullable) gets m + log(sum).  q is not rounded: scores
- * and sums carry fp32 (24 bits of q and of the probabilities).  The cells' order
- * of summation follows the lengths of the whole batch; the same call gives the
- * same bits.  A row that sees nothing (length 0) is 0, its lse -INFINITY; a row
+ * m the largest s_j and h / (n_head / n_head_kv) the K/V head (any whole ratio;
+ * n_head < 4096, n_rows < 2^24, scale > 0 and finite).  lse [n_rows][n_head]
+ * (nullable) gets m + log(sum).  q is not rounded to the cache's type: at least 22
+ * bits of it and of the probabilities count, scores and sums are fp32.  The cells'
+ * order of summation follows the lengths of the whole batch; the same call gives
+ * the same bits.  A row that sees nothing (length 0) is 0, its lse -INFINITY; a row
  * with a negative length is padding and left as it was.  Cells outside a row's
- * range are not read; in the cells it sees, K and V are finite (a head that meets
- * an infinity or NaN there, or in its query, gets values that are not finite).  A sequence outside [0, n_seqs) leaves its row without
- * cells, a length beyond the table is cut to it, and the cells of a page outside
+ * range are not read.  K and V of the cells in it are finite: an infinity or NaN
+ * there makes the rows' heads that meet it infinite or NaN, one in a query that
+ * head alone.  A sequence outside [0, n_seqs) leaves its row without cells, a
+ * length beyond the table is cut to it, and the cells of a page outside
  * [0, n_pages) are not seen; each makes alb_device_error() report 4.  A prompt's
  * tokens may be rows too (their own lengths), each reading its cells anew.
  * Nothing depends on the lengths but the work, so a captured call replays with
  * new lengths, tables and queries in the same buffers.  workspace:
- * alb_paged_attn_workspace_bytes() bytes, 16-byte aligned, no state kept in it
- * between calls; calls that may overlap in time (other streams, two captured
+ * alb_paged_attn_workspace_bytes() bytes (about 8 MB, whatever the batch), 16-byte
+ * aligned, no state kept in it between calls; calls that may overlap in time (other streams, two captured
  * graphs replayed side by side) need one each.  q and out are 16-byte aligned. */
 ALB_API size_t alb_paged_attn_workspace_bytes(const alb_paged_kv * kv, int64_t n_rows, int32_t n_head);
 ALB_API int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, const alb_paged_kv * kv,
@@ -312,7 +314,7 @@ typedef struct {
  * bias_ids are skipped; ids >= n_vocab, lengths beyond history_stride (cut to
  * it), bias offsets outside [0, n_bias] (cut) and mask rows >= n_allow (no mask)
  * make alb_device_error() report 4.  Extends sample_none (sampler.cpp:34-36),
- * the reference's only sampler.  n_vocab <= 450000. */
+ * the reference's only sampler.  n_vocab <= 450000, rows < 2^24. */
 ALB_API int alb_logits_process(const float * logits, int64_t rows, int64_t n_vocab, int64_t stride,
                                const alb_logits_rules * rules, float * out, int64_t out_stride, int32_t * next_token,
                                void * stream);
