@@ -267,7 +267,7 @@ ALB_API int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, int
  * tokens may be rows too (their own lengths), each reading its cells anew.
  * Nothing depends on the lengths but the work, so a captured call replays with
  * new lengths, tables and queries in the same buffers.  workspace:
- * alb_paged_attn_workspace_bytes() bytes (about 8 MB, whatever the batch), 16-byte
+ * alb_paged_attn_workspace_bytes() bytes (up to 9 MB, whatever the batch), 16-byte
  * aligned, no state kept in it between calls; calls that may overlap in time (other streams, two captured
  * graphs replayed side by side) need one each.  q and out are 16-byte aligned. */
 ALB_API size_t alb_paged_attn_workspace_bytes(const alb_paged_kv * kv, int64_t n_rows, int32_t n_head);
