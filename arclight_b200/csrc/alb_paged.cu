@@ -553,7 +553,9 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             float x[R][SUB][4];   // scores of cells 16 b + 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
             for (int b = 0; b < SUB; ++b) {
-                float s[2][4];
+                // Each product truncates its sums, so the small parts are summed apart from the first: in rows
+                // 8-15 (R = 1), in sums of their own (R = 2).
+                float s[2][4], small[2][4];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -566,21 +568,22 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
                             for (int p = 0; p < PARTS - 1; ++p) {
                                 const uint4 y = sq[warp][2 * p][k][lane], z = sq[warp][2 * p + 1][k][lane];
-                                pa_mma<BF16>(s[u], y.x, z.x, y.y, z.y, w.x, w.y);
-                                pa_mma<BF16>(s[u], y.z, z.z, y.w, z.w, w.z, w.w);
+                                if (k == 0 && p == 0) pa_mma0<BF16>(small[u], y.x, z.x, y.y, z.y, w.x, w.y);
+                                else                  pa_mma<BF16>(small[u], y.x, z.x, y.y, z.y, w.x, w.y);
+                                pa_mma<BF16>(small[u], y.z, z.z, y.w, z.w, w.z, w.w);
                             }
                         } else if (REST) {
                             const uint4 y = sq[warp][0][k][lane];
-                            pa_mma<BF16>(s[u], y.x, 0u, y.y, 0u, w.x, w.y);
-                            pa_mma<BF16>(s[u], y.z, 0u, y.w, 0u, w.z, w.w);
+                            pa_mma<BF16>(s[u], 0u, y.x, 0u, y.y, w.x, w.y);
+                            pa_mma<BF16>(s[u], 0u, y.z, 0u, y.w, w.z, w.w);
                         }
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     if (R == 2) {
-                        x[0][b][u] = s[u >> 1][u & 1];
-                        x[R - 1][b][u] = s[u >> 1][2 + (u & 1)];
+                        x[0][b][u] = s[u >> 1][u & 1] + small[u >> 1][u & 1];
+                        x[R - 1][b][u] = s[u >> 1][2 + (u & 1)] + small[u >> 1][2 + (u & 1)];
                     } else {
                         x[0][b][u] = s[u >> 1][u & 1] + s[u >> 1][2 + (u & 1)];
                     }
@@ -633,7 +636,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-                    float r[4];
+                    float r[4], small[4];
 #pragma unroll
                     for (int b = 0; b < SUB; ++b) {
                         auto word = [&](int u) { return reinterpret_cast<const uint32_t *>(&V[b][u][h])[j >> 1]; };
@@ -642,8 +645,9 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
                             for (int p = 0; p < PARTS; ++p) {
                                 uint32_t (& y)[SUB][2] = part[p][0], (& z)[SUB][2] = part[p][R - 1];
-                                if (b == 0 && p == 0) pa_mma0<BF16>(r, y[b][0], z[b][0], y[b][1], z[b][1], b0, b1);
-                                else                  pa_mma<BF16>(r, y[b][0], z[b][0], y[b][1], z[b][1], b0, b1);
+                                float (& sum)[4] = p == 0 ? r : small;
+                                if (b == 0 && p < 2) pa_mma0<BF16>(sum, y[b][0], z[b][0], y[b][1], z[b][1], b0, b1);
+                                else                 pa_mma<BF16>(sum, y[b][0], z[b][0], y[b][1], z[b][1], b0, b1);
                             }
                         } else {
                             const uint32_t y0 = FOUR && g >= 4 ? part[1][0][b][0] : part[0][0][b][0];
@@ -652,12 +656,12 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                             const uint32_t z1 = !FOUR ? part[1][0][b][1] : g < 4 ? part[PARTS - 1][0][b][1] : 0u;
                             if (b == 0) pa_mma0<BF16>(r, y0, z0, y1, z1, b0, b1);
                             else        pa_mma<BF16>(r, y0, z0, y1, z1, b0, b1);
-                            if (REST) pa_mma<BF16>(r, part[PARTS - 1][0][b][0], 0u, part[PARTS - 1][0][b][1], 0u, b0, b1);
+                            if (REST) pa_mma<BF16>(r, 0u, part[PARTS - 1][0][b][0], 0u, part[PARTS - 1][0][b][1], b0, b1);
                         }
                     }
                     if (R == 2) {
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) o[h][j][p & (2 * R - 1)] = fmaf(o[h][j][p & (2 * R - 1)], fix[(p >> 1) & (R - 1)], r[p]);
+                        for (int p = 0; p < 4; ++p) o[h][j][p & (2 * R - 1)] = fmaf(o[h][j][p & (2 * R - 1)], fix[(p >> 1) & (R - 1)], r[p] + small[p]);
                     } else {
                         o[h][j][0] = fmaf(o[h][j][0], fix[0], r[0] + r[2]);
                         o[h][j][1] = fmaf(o[h][j][1], fix[0], r[1] + r[3]);
