@@ -198,7 +198,7 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // products and keeps the third parts of q in shared memory: 64 sequences of 4k to
 // 8k cells 5.3 TB/s (4.3 with all parts in registers, which spill), where four
 // heads stream 6.6.  Units of 16 heads take one product a part of all 16: 200
-// sequences of 4k to 8k cells with 16 / 1 heads 129 us in fp16, 4.8 TB/s, and 157
+// sequences of 4k to 8k cells with 16 / 1 heads 136 us in fp16, 4.6 TB/s, and 153
 // in bf16 (two units of eight, which read K and V twice: 183 and 226).  A warp has a tile of K and V
 // (8 KB) in flight while it works on the one before, twelve warps an SM 96 KB; 16
 // warps at 128 registers spill (907 us), eight at 255 hold too little (676 us).  K
@@ -553,17 +553,19 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
             float x[R][SUB][4];   // scores of cells 16 b + 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
             for (int b = 0; b < SUB; ++b) {
-                // Each product truncates its sums, so the small parts are summed apart from the first: in rows
-                // 8-15 (R = 1), in sums of their own (R = 2).
-                float s[2][4], small[2][4];
+                // Each product truncates its sums, so the small parts are summed apart from the first (in rows
+                // 8-15 for R = 1, in sums of their own for R = 2), and chains are short: the worst of 6000 random
+                // cases is 6e-7 off, with one chain a row 1.8e-6.
+                float s[2][2][4], small[2][4];   // (two chains each, halves of the k steps)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
 #pragma unroll
                     for (int k = 0; k < KL; ++k) {
                         const uint4 & w = K[b][u][k];
-                        if (k == 0) pa_mma0<BF16>(s[u], qa[k][0], qb[k][0], qa[k][1], qb[k][1], w.x, w.y);
-                        else        pa_mma<BF16>(s[u], qa[k][0], qb[k][0], qa[k][1], qb[k][1], w.x, w.y);
-                        pa_mma<BF16>(s[u], qa[k][2], qb[k][2], qa[k][3], qb[k][3], w.z, w.w);
+                        float (& sum)[4] = s[k & 1][u];
+                        if (k < 2) pa_mma0<BF16>(sum, qa[k][0], qb[k][0], qa[k][1], qb[k][1], w.x, w.y);
+                        else       pa_mma<BF16>(sum, qa[k][0], qb[k][0], qa[k][1], qb[k][1], w.x, w.y);
+                        pa_mma<BF16>(sum, qa[k][2], qb[k][2], qa[k][3], qb[k][3], w.z, w.w);
                         if (R == 2) {
 #pragma unroll
                             for (int p = 0; p < PARTS - 1; ++p) {
@@ -574,18 +576,20 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                             }
                         } else if (REST) {
                             const uint4 y = sq[warp][0][k][lane];
-                            pa_mma<BF16>(s[u], 0u, y.x, 0u, y.y, w.x, w.y);
-                            pa_mma<BF16>(s[u], 0u, y.z, 0u, y.w, w.z, w.w);
+                            pa_mma<BF16>(sum, 0u, y.x, 0u, y.y, w.x, w.y);
+                            pa_mma<BF16>(sum, 0u, y.z, 0u, y.w, w.z, w.w);
                         }
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
+                    const float (& s0)[4] = s[0][u >> 1], (& s1)[4] = s[1][u >> 1];
+                    const int p = u & 1;
                     if (R == 2) {
-                        x[0][b][u] = s[u >> 1][u & 1] + small[u >> 1][u & 1];
-                        x[R - 1][b][u] = s[u >> 1][2 + (u & 1)] + small[u >> 1][2 + (u & 1)];
+                        x[0][b][u] = (s0[p] + s1[p]) + small[u >> 1][p];
+                        x[R - 1][b][u] = (s0[2 + p] + s1[2 + p]) + small[u >> 1][2 + p];
                     } else {
-                        x[0][b][u] = s[u >> 1][u & 1] + s[u >> 1][2 + (u & 1)];
+                        x[0][b][u] = (s0[p] + s1[p]) + (s0[2 + p] + s1[2 + p]);
                     }
                 }
             }
