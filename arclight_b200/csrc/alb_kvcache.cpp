@@ -530,6 +530,22 @@ int alb_kv_visible_cells(const alb_kv_cache * kv, int32_t seq_id, int32_t pos, u
     return ALB_OK;
 }
 
+int alb_kv_position_cells(const alb_kv_cache * kv, int32_t seq_id, int32_t p0, int32_t n, int32_t * cells_out) {
+    if (!kv || !cells_out || seq_id < 0 || seq_id >= (int32_t)kv->seq_to_stream.size() || p0 < 0 || n <= 0 ||
+        (int64_t)p0 + n > INT32_MAX)
+        return fail(ALB_ERR_INVALID, "kv: bad position-cells arguments");
+    if ((int64_t)kv->n_stream * kv->size > INT32_MAX)
+        return fail(ALB_ERR_INVALID, "kv: cell indices do not fit 32 bits");
+    const uint32_t st = kv->seq_to_stream[seq_id];
+    const Cells & c = kv->cells[st];
+    for (auto it = c.at[seq_id].lower_bound(p0); it != c.at[seq_id].end() && it->first < p0 + n; ++it)
+        if (it->second > 1) return fail(ALB_ERR_INVALID, "kv: two cells of the sequence hold one position");
+    for (int32_t i = 0; i < n; ++i) cells_out[i] = -1;
+    for (uint32_t j : c.used)
+        if (c.has(j, seq_id) && c.pos_in(j, p0, p0 + n)) cells_out[c.pos[j] - p0] = (int32_t)(st * kv->size + j);
+    return ALB_OK;
+}
+
 int alb_kv_cell(const alb_kv_cache * kv, uint32_t stream, uint32_t cell, int32_t * pos, uint64_t * seqs,
                 int32_t * shift) {
     if (!kv || stream >= kv->n_stream || cell >= kv->size) return fail(ALB_ERR_INVALID, "kv: bad cell");

@@ -119,13 +119,22 @@ class KVCache:
 
     def visible_cells(self, seq_id: int, pos: int, n_kv: int | None = None) -> np.ndarray:
         """Flat indices of the cells (seq_id, pos) may see among the first n_kv,
-        ascending: one mask row as a list (the rows to gather for attention)."""
+        ascending: one mask row as a list (the rows to gather for attention; not in
+        the order of the positions, see position_cells)."""
         n_kv = self.n_kv if n_kv is None else n_kv
         out = np.zeros(max(n_kv, 1), dtype=np.int64)
         n = C.c_int32()
         check(self._L.alb_kv_visible_cells(self._h, seq_id, pos, n_kv, out.ctypes.data, C.byref(n)),
               "alb_kv_visible_cells")
         return out[:n.value].copy()
+
+    def position_cells(self, seq_id: int, n: int, p0: int = 0) -> np.ndarray:
+        """Flat indices (int32) of the cells that hold positions p0 .. p0 + n - 1 of
+        the sequence, -1 where there is none: from p0 = 0 a page table row of the
+        paged operators with one-cell pages."""
+        out = np.empty(max(n, 1), dtype=np.int32)
+        check(self._L.alb_kv_position_cells(self._h, seq_id, p0, n, out.ctypes.data), "alb_kv_position_cells")
+        return out
 
     def cell(self, stream: int, idx: int) -> tuple[int, int, int]:
         """(position or -1, sequence bit set, accumulated shift) of one cell."""

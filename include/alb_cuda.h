@@ -203,8 +203,9 @@ ALB_API int alb_flash_attn_static(const float * q, const uint16_t * k_cache, con
 /* --------------------------------------------------------- paged K/V cache
  * A batch of sequences in one cache of fixed-size pages.  The cell of position p
  * of sequence s is slot p % page_size of page page_table[s][p / page_size]; with
- * page_size 1 the table holds cell indices, e.g. those of the KV-cache manager
- * (alb_kv_visible_cells).  No counterpart in the reference, whose cache is one
+ * page_size 1 the table holds the cell of each position, e.g. those of the
+ * KV-cache manager (alb_kv_position_cells; alb_kv_visible_cells lists them in
+ * another order).  No counterpart in the reference, whose cache is one
  * row of cells per stream with a dense mask (cgraph.cpp:1057-1261). */
 enum {
     ALB_KV_F16 = 0,

@@ -85,9 +85,20 @@ ALB_API int alb_kv_mask(const alb_kv_cache * kv, const int32_t * pos, const int3
 /* One row of that mask as a list: the flat indices (stream * kv_size + cell,
  * ascending) of the cells j < n_kv that query (seq_id, pos) may see, into
  * cells_out (room for n_kv); *n_out = their count.  Gathering those K/V rows
- * (alb_get_rows_f16) gives the contiguous cache alb_flash_attn takes. */
+ * (alb_get_rows_f16) gives the contiguous cache alb_flash_attn takes.  The
+ * order is that of the cells, not of the positions: no page table row. */
 ALB_API int alb_kv_visible_cells(const alb_kv_cache * kv, int32_t seq_id, int32_t pos, uint32_t n_kv,
                                  int64_t * cells_out, int32_t * n_out);
+/* The sequence's cells by position: cells_out[i] = flat index of the cell that
+ * holds position p0 + i (0 <= i < n), -1 where the sequence holds no such
+ * position.  Positions from 0 on make a row of alb_paged_kv's page table with
+ * page_size 1 (n_pages = n_stream * kv_size), whatever order the cells were
+ * handed out in and after seq_rm and seq_add too; positions that were removed and
+ * not closed up stay -1, a page that the paged operators report.  Refused
+ * when two cells of the sequence hold one of the positions (a row of a table
+ * names one), or a flat index does not fit 32 bits. */
+ALB_API int alb_kv_position_cells(const alb_kv_cache * kv, int32_t seq_id, int32_t p0, int32_t n,
+                                  int32_t * cells_out);
 /* Inspection: cell `cell` of stream `stream`: its position (-1 empty), the
  * bit set of its sequences and its accumulated shift. */
 ALB_API int alb_kv_cell(const alb_kv_cache * kv, uint32_t stream, uint32_t cell, int32_t * pos, uint64_t * seqs,

@@ -1,0 +1,75 @@
+"""Paged append and attention where test_gpu_paged.py does not reach: tables of
+the cell manager, values at the ends of their types, each part of the split
+queries and probabilities by itself, every way to deal heads out to units.
+Tolerances are test_gpu_paged.py's unless a test derives its own."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+import arclight_b200 as A
+from arclight_b200.kvcache import KVCache
+from tests import test_gpu_paged as P
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F16, BF16 = A.ALB_KV_F16, A.ALB_KV_BF16
+L = None
+
+
+def setup_module():
+    global L
+    P.setup_module()
+    L = P.L
+
+
+def i32(a):
+    return torch.as_tensor(a, dtype=torch.int32, device="cuda")
+
+
+# ----------------------------------------------------------------------------------- tables of the cell manager
+@pytest.mark.parametrize("typ", [F16, BF16], ids=["f16", "bf16"])
+def test_tables_of_a_manager_whose_slots_wrapped(typ):
+    """Freed cells are taken again, so cells and positions are in different orders:
+    appends, a sliding window and a prompt's causal rows by position."""
+    heads, hkv, dim, n = 8, 2, 128, 20
+    kv = KVCache(32, 2, True, 32)
+    dg = torch.Generator(device="cuda").manual_seed(7 + typ)
+    x = torch.randn(n, heads + 2 * hkv, dim, generator=dg, device="cuda")
+    rope = P.angles(64, dim)
+    (slot,) = kv.prepare([(np.arange(16), np.zeros(16))])
+    kv.apply(np.arange(16), np.zeros(16), slot)          # sequence 0 holds cells 0 .. 15, then leaves
+    cache = P.Cache(32, 1, hkv, dim, typ, torch.full((2, n), -1))
+    L.alb_device_error(1)
+    q = torch.empty(n, heads, dim, device="cuda")
+    for first, last in [(0, 10)] + [(p, p + 1) for p in range(10, n)]:
+        if first == 10:
+            kv.seq_rm(0, -1, -1)
+        pos = np.arange(first, last)
+        (slot,) = kv.prepare([(pos, np.ones(len(pos)))])
+        kv.apply(pos, np.ones(len(pos)), slot)
+        cache.table[1].copy_(i32(kv.position_cells(1, n)))
+        P.append(cache, x[first:last].reshape(last - first, -1), heads, None, None, rope, i32(pos),
+                 i32(np.ones(len(pos))), q=q[first:last])
+        assert all(int(cache.table[1, p]) == int(c) for p, c in zip(pos, slot))
+    cells = cache.table[1].tolist()
+    assert sorted(cells) == sorted(kv.visible_cells(1, n - 1, 32)) and cells != sorted(cells)
+    # position p's rows lie in its cell
+    k, v = cache.rows(1, 0, n)
+    assert torch.equal(v, x[:, heads + hkv:].to(P.DT[typ]).double().cpu())
+    want, tol = P.rotated(x[:, heads:heads + hkv], None, rope, torch.arange(n))
+    half = torch.finfo(P.DT[typ]).eps / 2
+    assert torch.all((k - want).abs() <= tol + half * want.abs() * (1 + 2 ** -10) + 2.0 ** -25)
+    for window in (0, 5):
+        out, lse = P.attend(cache, q, i32(range(1, n + 1)), i32([1] * n), window=window)
+        P.check_rows(cache, q, list(range(1, n + 1)), out, lse, seqs=[1] * n, window=window)
+    # the front goes and the rest closes up: rows are read by their new positions
+    kv.seq_rm(1, 0, 6)
+    kv.seq_add(1, 6, -1, -6)
+    cache.table[1].copy_(i32(kv.position_cells(1, n)))
+    out, lse = P.attend(cache, q[:1], i32([n - 6]), i32([1]), window=4)
+    P.check_rows(cache, q[:1], [n - 6], out, lse, seqs=[1], window=4)
+    assert torch.equal(cache.rows(1, 0, n - 6)[1], v[6:])
+    assert L.alb_device_error(0) == 0

@@ -172,3 +172,78 @@ def test_visible_cells_are_the_mask_rows(cfg):
             row = kv.set_inputs_attn_mask([p], [s], 1, kv.kv_size)[0, 0]
             want = st * kv.kv_size + np.nonzero(row == 0)[0]
             assert np.array_equal(kv.visible_cells(s, p, kv.kv_size), want)
+
+
+def _wrapped():
+    """32 cells in which sequence 1's positions 0..9 lie at cells 16..25 and 10..19 at 0..9."""
+    kv = KVCache(32, 2, True, 32)
+    for seq, first, n in ((0, 0, 16), (1, 0, 10)):
+        pos = np.arange(first, first + n)
+        (slot,) = kv.prepare([(pos, np.full(n, seq))])
+        kv.apply(pos, np.full(n, seq), slot)
+    kv.seq_rm(0, -1, -1)
+    for p in range(10, 20):
+        (slot,) = kv.prepare([([p], [1])])
+        kv.apply([p], [1], slot)
+    return kv
+
+
+def test_position_cells_of_a_cache_whose_slots_wrapped():
+    """A table row names the cell of each position; the list of visible cells does not."""
+    kv = _wrapped()
+    row = kv.position_cells(1, 20)
+    assert [kv.cell(0, int(c))[0] for c in row] == list(range(20))
+    visible = kv.visible_cells(1, 19, 32)
+    assert sorted(row) == list(visible) and list(row) != list(visible)
+    assert list(kv.position_cells(1, 3, p0=8)) == list(row[8:11])
+    assert list(kv.position_cells(1, 5, p0=18)) == [row[18], row[19], -1, -1, -1]
+    assert list(kv.position_cells(0, 4)) == [-1] * 4
+    # a front part goes, what is left closes up
+    kv.seq_rm(1, 0, 4)
+    assert list(kv.position_cells(1, 20)) == [-1] * 4 + list(row[4:])
+    kv.seq_add(1, 4, -1, -4)
+    assert list(kv.position_cells(1, 17)) == list(row[4:]) + [-1]
+
+
+@pytest.mark.parametrize("unified", [True, False])
+def test_position_cells_follow_random_use(unified):
+    rng = np.random.default_rng(5)
+    kv = KVCache(64, 4, unified, 32)
+    for _ in range(300):
+        s = int(rng.integers(0, 4))
+        lo, hi = kv.seq_pos_min(s), kv.seq_pos_max(s)
+        kind = rng.integers(0, 8)
+        if kind == 0 and hi >= 0:
+            kv.seq_rm(s, int(rng.integers(lo, hi + 1)), -1)
+        elif kind == 1 and hi > 0:
+            kv.seq_rm(s, lo, int(rng.integers(lo, hi + 1)))
+        elif kind == 2 and lo > 0:
+            kv.seq_add(s, lo, -1, -int(rng.integers(1, lo + 1)))
+        else:
+            pos = np.arange(hi + 1, hi + 1 + int(rng.integers(1, 6)))
+            slots = kv.prepare([(pos, np.full(len(pos), s))])
+            if slots:
+                kv.apply(pos, np.full(len(pos), s), slots[0])
+        for q in range(4):
+            hi, st = kv.seq_pos_max(q), 0 if unified else q
+            want = np.full(hi + 3, -1)
+            for j in range(64):
+                p, seqs, _ = kv.cell(st, j)
+                if p >= 0 and seqs >> q & 1:
+                    want[p] = st * 64 + j
+            np.testing.assert_array_equal(kv.position_cells(q, hi + 3), want)
+
+
+def test_position_cells_refusals():
+    kv = _wrapped()
+    L, out = A.lib(), np.full(4, 7, np.int32)
+    for h, seq, p0, n, o in ((None, 1, 0, 4, out.ctypes.data), (kv._h, -1, 0, 4, out.ctypes.data),
+                             (kv._h, 64, 0, 4, out.ctypes.data), (kv._h, 1, -1, 4, out.ctypes.data),
+                             (kv._h, 1, 0, 0, out.ctypes.data), (kv._h, 1, 0, -3, out.ctypes.data),
+                             (kv._h, 1, 2 ** 31 - 4, 4, out.ctypes.data), (kv._h, 1, 0, 4, None)):
+        assert L.alb_kv_position_cells(h, seq, p0, n, o) == A.ALB_ERR_INVALID
+    # two cells of one position: no row can name both
+    kv.seq_add(1, 0, 1, 1)
+    assert L.alb_kv_position_cells(kv._h, 1, 0, 4, out.ctypes.data) == A.ALB_ERR_INVALID
+    assert (out == 7).all()
+    assert L.alb_kv_position_cells(kv._h, 1, 2, 2, out.ctypes.data) == A.ALB_OK
