@@ -189,8 +189,12 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // which a long chain would gather into a bias.
 //
 // Exponents are base 2 and the running maximum is rounded up to a whole number,
-// so rescaling is exact; probabilities are scaled by 2^15 to stay clear of fp16's
-// subnormals (p >= 2^-24 of the largest keeps its leading part normal).
+// so rescaling is exact.  fp16 probabilities are scaled by 2^15 to stay clear of
+// fp16's subnormals (p >= 2^-24 of the largest keeps its leading part normal).
+// bf16 has fp32's exponents: its values may be as large as the sums can be, so its
+// probabilities are scaled by 2^-k where a row has at most 2^k cells (table and
+// window say so), and no sum passes the largest |V|; q is scaled below 2^-9, so
+// that 128 products with any K fit too.
 //
 // Bound by HBM: 48 sequences of 8k to 32k cells (32 / 8 heads of 128) stream 4.2 GB
 // in 622 us, 6.75 TB/s; 37 ragged ones 110 us (bf16, its three parts in one
@@ -217,7 +221,8 @@ template <int D> constexpr int PA_TILE = 16 * 128 / D;
 constexpr int PA_MAX_CTAS = 1024;        // of units of 8 heads; of 16: half as many
 constexpr int PA_MIN_TILES = 4;          // a CTA's range is at least a tile per warp
 constexpr int PA_SETUP = 6;              // what a unit costs beside its tiles, in tiles
-constexpr float PA_SHIFT = 15.0f;
+template <bool BF16> constexpr float PA_SHIFT = BF16 ? 0.0f : 15.0f;     // of the probabilities' exponents
+template <bool BF16> constexpr int PA_Q_EXP = BF16 ? -10 : 9;            // of a row of q's largest value
 
 // What each CTA left unfinished: the unit that its range began and did not end
 // (its tail; row -1: none), and whether the unit that its range began inside of
@@ -237,6 +242,7 @@ struct PaArgs {
     int64_t n_rows;
     int32_t Hq, G, groups, window;
     float scale_log2;
+    float p_scale;       // what probabilities and their sums are scaled by: 2^PA_SHIFT (fp16), 2^-k
     PaMeta * meta;
     float * pieces;
     float * out, * lse;
@@ -267,6 +273,9 @@ template <int TILE> __device__ __forceinline__ int32_t pa_weight(const PaArgs & 
     const int32_t n = pa_tiles<TILE>(a, r);
     return n ? n + PA_SETUP : 0;
 }
+
+// 1 / p_scale, both powers of two.
+__device__ __forceinline__ float pa_unscale(const PaArgs & a) { return __uint_as_float(0x7f000000u - __float_as_uint(a.p_scale)); }
 
 __device__ __forceinline__ float pa_ex2(float x) {
     float y;
@@ -508,10 +517,11 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                 for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(qv[r][i][e]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^e with top 2^e in [2^9, 2^10); nothing to scale for 0 and what is not finite
+            // 2^e with top 2^e in [1, 2) 2^PA_Q_EXP; nothing to scale for 0 and what is not finite
             const int ex = (int)(__float_as_uint(top) >> 23);           // biased exponent, 0 for subnormals
-            int e = ex == 255 || top == 0.0f ? 0 : 127 + 9 - max(ex, 1);
+            int e = ex == 255 || top == 0.0f ? 0 : 127 + PA_Q_EXP<BF16> - max(ex, 1);
             e = min(e, 126);
+            if (BF16) e = max(e, -126);   // (at least -118 with fp16)
             const float up = __uint_as_float((uint32_t)(e + 127) << 23);
             c[r] = e > 0 ? a.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) : a.scale_log2 * (1.0f / up);
 #pragma unroll
@@ -625,7 +635,10 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                     float (& y)[4] = x[r][b];
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
-                        y[u] = !ok[b][u] ? 0.0f : pa_ex2(big ? __fmul_rn(y[u], c[r]) - base + PA_SHIFT : fmaf(y[u], c[r], PA_SHIFT - base));
+                        y[u] = !ok[b][u] ? 0.0f : pa_ex2(big ? __fmul_rn(y[u], c[r]) - base + PA_SHIFT<BF16> : fmaf(y[u], c[r], PA_SHIFT<BF16> - base));
+                    if (BF16)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) y[u] *= a.p_scale;
                     l[r] += (y[0] + y[1]) + (y[2] + y[3]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
@@ -734,7 +747,7 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
                         *reinterpret_cast<float4 *>(dst + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
                     if (a.lse && d == 0)
                         a.lse[(int64_t)row * a.Hq + head0 + h] =
-                            Ls != 0.0f ? fmaf(M, 0.693147181f, logf(Ls * 0x1p-15f)) : -INFINITY;
+                            Ls != 0.0f ? fmaf(M, 0.693147181f, logf(Ls * (BF16 ? pa_unscale(a) : 0x1p-15f))) : -INFINITY;
                 } else {
                     float * piece = a.pieces + (2 * cta + (begins ? 1 : 0)) * pa_piece_floats<D, R>() + h * D + d;
 #pragma unroll
@@ -857,7 +870,7 @@ k_paged_attn_join(const __grid_constant__ PaArgs a) {
 #pragma unroll
             for (int e = 0; e < N; ++e) acc[e] = L != 0.0f ? acc[e] / L : 0.0f;
             *reinterpret_cast<F *>(a.out + head * D + N * lane) = *reinterpret_cast<F *>(acc);
-            if (a.lse && lane == 0) a.lse[head] = L != 0.0f ? fmaf(top, 0.693147181f, logf(L * 0x1p-15f)) : -INFINITY;
+            if (a.lse && lane == 0) a.lse[head] = L != 0.0f ? fmaf(top, 0.693147181f, logf(L * pa_unscale(a))) : -INFINITY;
         }
     }
     alb_pdl_trigger();
@@ -955,7 +968,12 @@ cudaError_t launch_attn_r(PaArgs a, cudaStream_t st) {
 }
 
 template <int D, bool BF16>
-cudaError_t launch_attn(const PaArgs & a, cudaStream_t st) {
+cudaError_t launch_attn(PaArgs a, cudaStream_t st) {
+    int64_t most = (int64_t)a.kv.max_pages * a.kv.page_size;
+    if (a.window > 0 && a.window < most) most = a.window;
+    int k = 0;
+    while (BF16 && ((int64_t)1 << k) < most) ++k;
+    a.p_scale = std::ldexp(1.0f, (int)PA_SHIFT<BF16> - k);
     // more than 8 heads a group: units of 16, which read K and V once
     if (a.G > 8) return launch_attn_r<D, BF16, false, 2>(a, st);
     return BF16 && a.G <= 4 ? launch_attn_r<D, BF16, BF16, 1>(a, st) : launch_attn_r<D, BF16, false, 1>(a, st);

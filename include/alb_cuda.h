@@ -260,9 +260,10 @@ ALB_API int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, int
  * order of summation follows the lengths of the whole batch; the same call gives
  * the same bits.  A row that sees nothing (length 0) is 0, its lse -INFINITY; a row
  * with a negative length is padding and left as it was.  Cells outside a row's
- * range are not read.  K and V of the cells in it are finite: an infinity or NaN
- * there makes the rows' heads that meet it infinite or NaN, one in a query that
- * head alone.  A sequence outside [0, n_seqs) leaves its row without cells, a
+ * range are not read.  K and V of the cells in it are finite, up to the ends of
+ * their type, scores and scale * |q| below 1e34: an infinity or NaN in K or V makes
+ * the rows' heads that meet it infinite or NaN, one in a query that head alone.
+ * (bf16 values are held to an absolute 1e-44 per position of the table or window too.)  A sequence outside [0, n_seqs) leaves its row without cells, a
  * length beyond the table is cut to it, and the cells of a page outside
  * [0, n_pages) are not seen; each makes alb_device_error() report 4.  A prompt's
  * tokens may be rows too (their own lengths), each reading its cells anew.

@@ -73,3 +73,32 @@ def test_tables_of_a_manager_whose_slots_wrapped(typ):
     P.check_rows(cache, q[:1], [n - 6], out, lse, seqs=[1], window=4)
     assert torch.equal(cache.rows(1, 0, n - 6)[1], v[6:])
     assert L.alb_device_error(0) == 0
+
+
+# --------------------------------------------------------------------------------------- values at the types' ends
+@pytest.mark.parametrize("lens", [[1, 2, 15, 33, 300, 5000], [40000]], ids=["batch", "one"])
+@pytest.mark.parametrize("heads,hkv,dim", [(4, 1, 128), (8, 1, 128), (2, 2, 64), (6, 1, 64), (16, 1, 128), (17, 1, 64)])
+def test_bf16_values_over_the_whole_type(heads, hkv, dim, lens):
+    """Finite K and V give finite results up to the type's end: a mean of values lies
+    among them, and scores that fit are made of large and small factors."""
+    top = torch.finfo(torch.bfloat16).max
+    gen = torch.Generator().manual_seed(heads + dim)
+    dg = torch.Generator(device="cuda").manual_seed(heads + dim + len(lens))
+    table, pool = P.make_table(lens, 16, gen)
+    cache = P.Cache(pool, 16, hkv, dim, BF16, table)
+    q = torch.randn(len(lens), heads, dim, generator=dg, device="cuda")
+    n = i32(lens)
+    for k_size, q_size in ((1.0, 1.0), (1e36, 1e-36), (7e37, 1e-37), (1e-36, 1e36)):
+        for s, m in enumerate(lens):
+            cache.fill(s, m, dg)
+        cache.k.copy_((cache.k.float() * k_size).clamp(-top, top))
+        v = cache.v.float()
+        v[..., 0::4] = torch.where(v[..., 0::4].isnan(), v[..., 0::4], top)               # the end itself
+        v[..., 1::4] = torch.copysign(torch.where(v[..., 1::4].isnan(), v[..., 1::4], top), v[..., 1::4])
+        v[..., 2::4] *= 1e35
+        v[..., 3::4] *= 1e-30
+        cache.v.copy_(v)
+        out, lse = P.attend(cache, q * q_size, n)
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+        P.check_rows(cache, q * q_size, lens, out, lse)
+        assert torch.allclose(out[..., 0::4], torch.tensor(top, device="cuda"), rtol=2.0 ** -18)
