@@ -239,7 +239,8 @@ k_logits(const __grid_constant__ LogitsArgs a) {
             // largest place wins the table entry; its thread leaves x + bias in y and a mark that
             // keeps earlier entries away
             int32_t b0 = r.bias_offsets[row], b1 = r.bias_offsets[row + 1];
-            if (b0 < 0 || b1 > r.n_bias) { bad = true; b0 = max(b0, 0); b1 = min(b1, r.n_bias); }
+            // (in order and inside the list: 0 <= b0 <= b1 <= n_bias)
+            if (b0 < 0 || b1 > r.n_bias || b0 > b1) { bad = true; b0 = max(b0, 0); b1 = min(b1, r.n_bias); }
             for (int32_t end = b1; end > b0; end -= LG_THREADS) {
                 const int32_t e = end - 1 - tid;
                 const uint32_t place = LG_THREADS - tid;

@@ -354,3 +354,21 @@ def test_division_by_the_temperature_rounds_as_the_quotient():
         want = x / temps[:, None]
     np.testing.assert_array_equal(y.view(np.uint32), want.view(np.uint32))
     np.testing.assert_array_equal(n, want.argmax(1))
+
+
+@pytest.mark.parametrize("offsets", [(900, 4, 4), (0, -5, 0), (-9, -5, -1), (5, 9, 900), (2, 1, 4), (0, 2 ** 31 - 1, -2 ** 31)])
+def test_bias_offsets_outside_the_list_or_falling_are_reported(offsets):
+    """Starts and ends on either side of the list, and ranges that run backwards: what lies in the list counts."""
+    X, Y = torch.zeros(2, 50, device="cuda"), torch.zeros(2, 50, device="cuda")
+    off, ids, val = cu(np.array(offsets, np.int32)), cu(np.arange(4, dtype=np.int32)), cu(np.ones(4, F))
+    r = A.LogitsRules(bias_offsets=off.data_ptr(), bias_ids=ids.data_ptr(), bias_values=val.data_ptr(), n_bias=4)
+    for row in range(2):                     # each row alone, so that each reports
+        r.bias_offsets = off[row:].data_ptr()
+        L.alb_device_error(1)
+        A.check(L.alb_logits_process(X.data_ptr(), 1, 50, 0, C.byref(r), Y[row].data_ptr(), 0, None, st()))
+        torch.cuda.synchronize()
+        b0, b1 = offsets[row], offsets[row + 1]
+        assert L.alb_device_error(1) == (0 if 0 <= b0 <= b1 <= 4 else 4), (b0, b1)
+        want = np.zeros(50, F)
+        want[max(b0, 0):max(min(b1, 4), 0)] = 1
+        np.testing.assert_array_equal(Y[row].cpu().numpy(), want)
