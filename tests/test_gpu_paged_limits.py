@@ -102,3 +102,81 @@ def test_bf16_values_over_the_whole_type(heads, hkv, dim, lens):
         assert torch.isfinite(out).all() and torch.isfinite(lse).all()
         P.check_rows(cache, q * q_size, lens, out, lse)
         assert torch.allclose(out[..., 0::4], torch.tensor(top, device="cuda"), rtol=2.0 ** -18)
+
+
+# ----------------------------------------------------------------------------------------- the parts one by one
+KINDS = [(1, 1), (4, 1), (6, 2), (5, 1), (8, 1), (12, 1), (16, 1), (17, 1)]
+
+
+def parts(x, typ, n):
+    """x as the sum of its n leading parts in the cache's type."""
+    got = torch.zeros_like(x)
+    for _ in range(n):
+        got = got + (x - got).to(P.DT[typ]).to(x.dtype)
+    return got
+
+
+@pytest.mark.parametrize("typ", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,hkv", KINDS)
+def test_every_part_of_the_query_counts(heads, hkv, dim, typ):
+    """Rows of one cell whose K is 1 in one place d: lse is q_d itself (scale 1, 1 <= |q_d| < 2).
+
+    The score's parts add up without rounding (bf16: three hold all 24 bits; fp16: two leave 2^-23 at most).
+    x log2(e): the constant is 2^-26.2 off, 4e-8; the exponent 2^-25 (between -1 and 0; fp16: 2^-21, between 14
+    and 15); ex2 2^-22; ln 2 times those, the logarithm 2^-24 and the last sum 2^-24: 4.2e-7 < 2^-21 with bf16;
+    fp16 has 3.1e-7 + 2^-23 more: 8.5e-7 < 2^-20.
+    """
+    g = torch.Generator().manual_seed(heads * dim + typ)
+    q = (2 ** 23 + 2 * torch.randint(0, 2 ** 22, (dim, heads, dim), generator=g) + 1).double() / 2 ** 23
+    q = q * (1 - 2 * torch.randint(0, 2, q.shape, generator=g))
+    table = torch.arange(dim)[:, None]
+    cache = P.Cache(dim, 1, hkv, dim, typ, table)
+    cache.v.zero_()
+    cache.k.zero_()
+    at = torch.arange(dim)
+    cache.k[at, 0, :, at] = 1.0
+    _, lse = P.attend(cache, q.float().cuda(), i32([1] * dim), scale=1.0)
+    want = q[at, :, at]
+    tol = 2.0 ** -20 if typ == F16 else 2.0 ** -21
+    assert float((lse.double().cpu() - want).abs().max()) <= tol
+    # one part fewer lies outside
+    assert float((parts(want, typ, 1 if typ == F16 else 2) - want).abs().max()) > 4 * tol
+
+
+@pytest.mark.parametrize("typ", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,hkv", KINDS)
+def test_every_part_of_the_probabilities_counts(heads, hkv, dim, typ):
+    """Cell j's V is 1 in one place, so that value is its probability; its K is a_j in the first place and q_0 is
+    1, so its score a_j (-2 to 2) is exact.
+
+    A weight is off by the constant (4e-8), the exponent's rounding (-7 to 0: 2^-22; fp16 8 to 16: 2^-21), both
+    times ln 2, and ex2's 2^-22: 4.4e-7, fp16 6e-7.  Their sum adds eight roundings (2 in a tile, 2 among lanes, 4
+    warps) of 2^-24: 4.8e-7.  Three bf16 parts hold the weight, two fp16 parts leave 2^-23; the sum of the parts,
+    the rescaled sum and the quotient round: 1.8e-7.  Twice the weight's, then: 1.6e-6, fp16 2e-6 at most.
+    """
+    n = 40
+    g = torch.Generator().manual_seed(heads * dim + typ)
+    rows = 6
+    a = (torch.rand(rows, n, hkv, generator=g) * 4 - 2).to(P.DT[typ])
+    table = torch.arange(rows * 3).view(rows, 3)
+    cache = P.Cache(rows * 3, 16, hkv, dim, typ, table)
+    k = torch.zeros(rows, 48, hkv, dim, dtype=P.DT[typ])
+    v = torch.zeros_like(k)
+    k[:, :n, :, 0] = a
+    place = (torch.arange(n)[None] + 11 * torch.arange(rows)[:, None]) % dim
+    v[torch.arange(rows)[:, None], torch.arange(n)[None], :, place] = 1.0
+    cache.k.copy_(k.view(rows * 3, 16, hkv, dim))
+    cache.v.copy_(v.view(rows * 3, 16, hkv, dim))
+    q = torch.randn(rows, heads, dim, generator=g)
+    q[..., 0] = 1.0
+    out, _ = P.attend(cache, q.cuda(), i32([n] * rows), scale=1.0)
+    p = torch.softmax(a.double(), 1).repeat_interleave(heads // hkv, 2)            # [rows][n][heads]
+    want = torch.zeros(rows, heads, dim, dtype=torch.float64)
+    want[torch.arange(rows)[:, None], :, place] = p
+    tol = 2e-6 if typ == F16 else 1.6e-6
+    assert torch.all((out.double().cpu() - want).abs() <= tol * want)
+    # one part fewer lies outside (weights as the kernel has them, largest 1 or a power of two below)
+    w = torch.exp2(a.double() / math.log(2) - (a.double() / math.log(2)).amax(1, keepdim=True).ceil())
+    assert float(((parts(w, typ, 1 if typ == F16 else 2) - w).abs() / w).max()) > 2 * tol
