@@ -180,3 +180,54 @@ def test_every_part_of_the_probabilities_counts(heads, hkv, dim, typ):
     # one part fewer lies outside (weights as the kernel has them, largest 1 or a power of two below)
     w = torch.exp2(a.double() / math.log(2) - (a.double() / math.log(2)).amax(1, keepdim=True).ceil())
     assert float(((parts(w, typ, 1 if typ == F16 else 2) - w).abs() / w).max()) > 2 * tol
+
+
+# -------------------------------------------------------------------------------------- heads dealt out to units
+@pytest.mark.parametrize("typ", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("heads,hkv,dim,page,layout,window", [
+    (17, 1, 128, 16, "dense", 0),        # a unit of 16 heads and one of a single head
+    (17, 1, 64, 5, "heads", 100),
+    (40, 1, 64, 7, "head_major", 0),     # 16, 16 and 8
+    (40, 1, 128, 64, "joined", 17),
+    (48, 2, 128, 32, "dense", 0),        # 16 and 8 for each K/V head
+    (66, 2, 64, 1, "dense", 63),         # 16, 16 and 1
+    (24, 2, 128, 16, "dense", 129),      # one unit of 12
+    (16, 2, 64, 16, "heads", 16),        # eight
+    (12, 2, 128, 16, "dense", 65),       # six
+    (6, 2, 128, 1, "joined", 300),       # three
+])
+def test_units_and_windows(heads, hkv, dim, page, layout, window, typ):
+    gen = torch.Generator().manual_seed(heads * dim + page)
+    dg = torch.Generator(device="cuda").manual_seed(heads + typ)
+    lens = P.LENGTHS + [-1]
+    table, pool = P.make_table([max(0, n) for n in lens], page, gen)
+    cache = P.Cache(pool, page, hkv, dim, typ, table, layout)
+    for s, n in enumerate(lens):
+        if n > 0:
+            cache.fill(s, n, dg)
+    q = torch.randn(len(lens), heads, dim, generator=dg, device="cuda") * 2
+    L.alb_device_error(1)
+    out, lse = P.attend(cache, q, i32(lens), window=window)
+    assert L.alb_device_error(0) == 0
+    P.check_rows(cache, q, lens, out, lse, window=window)
+
+
+@pytest.mark.parametrize("heads,hkv,dim,typ", [
+    (4, 1, 128, BF16), (6, 1, 128, BF16), (8, 1, 128, F16), (16, 1, 128, F16), (16, 1, 64, BF16),
+    (17, 1, 128, BF16), (33, 1, 64, F16), (40, 2, 128, BF16),
+])
+def test_one_long_row_in_many_pieces(heads, hkv, dim, typ):
+    """Units cut into more pieces than a round of the join takes, then beside short rows."""
+    gen = torch.Generator().manual_seed(heads)
+    dg = torch.Generator(device="cuda").manual_seed(heads)
+    lens = [40000, 1, 700, 0]
+    table, pool = P.make_table(lens, 16, gen)
+    cache = P.Cache(pool, 16, hkv, dim, typ, table)
+    for s, n in enumerate(lens):
+        cache.fill(s, n, dg)
+    q = torch.randn(len(lens), heads, dim, generator=dg, device="cuda")
+    for rows in (1, 4):
+        out, lse = P.attend(cache, q[:rows], i32(lens[:rows]))
+        P.check_rows(cache, q[:rows], lens[:rows], out, lse)
+        out, lse = P.attend(cache, q[:rows], i32(lens[:rows]), window=30000)
+        P.check_rows(cache, q[:rows], lens[:rows], out, lse, window=30000)
