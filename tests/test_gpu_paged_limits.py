@@ -231,3 +231,88 @@ def test_one_long_row_in_many_pieces(heads, hkv, dim, typ):
         P.check_rows(cache, q[:rows], lens[:rows], out, lse)
         out, lse = P.attend(cache, q[:rows], i32(lens[:rows]), window=30000)
         P.check_rows(cache, q[:rows], lens[:rows], out, lse, window=30000)
+
+
+# ------------------------------------------------------------------------------------------- calls behind calls
+def test_a_call_reads_what_the_call_before_it_writes():
+    """Each kernel may start while the one before it still runs: the append's input comes from
+    the logits operator, the attention's cache from the append, without a wait between."""
+    T, heads, hkv, dim = 600, 8, 2, 128
+    wide = (heads + 2 * hkv) * dim
+    dg = torch.Generator(device="cuda").manual_seed(1)
+    cache = P.Cache(T, 1, hkv, dim, F16, torch.arange(T)[None])
+    rope, pos, seqs = P.angles(T, dim), i32(range(T)), i32([0] * T)
+    hist = torch.randint(0, wide, (T, 3000), generator=dg, device="cuda", dtype=torch.int32)
+    rep, temp = torch.full((T,), 1.2, device="cuda"), torch.full((T,), 0.7, device="cuda")
+    r = A.LogitsRules(history=hist.data_ptr(), history_stride=3000, repetition=rep.data_ptr(), temperature=temp.data_ptr())
+    qkv = torch.empty(T, wide, device="cuda")
+    lens = i32(range(1, T + 1))
+    bufs = [dict(q=torch.empty(T, heads, dim, device="cuda"), out=torch.empty(T, heads, dim, device="cuda"),
+                 lse=torch.empty(T, heads, device="cuda")) for _ in range(2)]
+    ws = torch.empty(L.alb_paged_attn_workspace_bytes(cache.ref(), T, heads), dtype=torch.uint8, device="cuda")
+    for _ in range(10):
+        x = torch.randn(T, wide, generator=dg, device="cuda")
+        kept = []
+        for wait, b in zip((False, True), bufs):
+            for t in (qkv, cache.k, cache.v, b["q"]):
+                t.fill_(100.0)               # a stale read shows
+            torch.cuda.synchronize()
+            A.check(L.alb_logits_process(x.data_ptr(), T, wide, 0, C.byref(r), qkv.data_ptr(), 0, None, P.st()))
+            if wait:
+                torch.cuda.synchronize()
+            A.check(L.alb_qk_norm_rope_kv_paged(qkv.data_ptr(), 0, T, heads, None, None, 1e-6, rope.data_ptr(), T,
+                                                pos.data_ptr(), seqs.data_ptr(), cache.ref(), b["q"].data_ptr(), P.st()))
+            if wait:
+                torch.cuda.synchronize()
+            A.check(L.alb_paged_attn(b["q"].data_ptr(), T, heads, cache.ref(), seqs.data_ptr(), lens.data_ptr(), 0,
+                                     dim ** -0.5, ws.data_ptr(), b["out"].data_ptr(), b["lse"].data_ptr(), P.st()))
+            torch.cuda.synchronize()
+            kept.append([t.clone() for t in (cache.k, cache.v, b["q"], b["out"], b["lse"])])
+        for a, b in zip(*kept):
+            assert torch.equal(a, b)
+
+
+def test_captured_calls_on_streams_that_fork_and_join():
+    """Two branches of one graph: append and logits side by side, the attention behind both."""
+    B, heads, hkv, dim, vocab = 5, 8, 2, 64, 5000
+    lens = [40, 1, 300, 17, 64]
+    gen = torch.Generator().manual_seed(2)
+    dg = torch.Generator(device="cuda").manual_seed(2)
+    table, pool = P.make_table(lens, 16, gen)
+    cache = P.Cache(pool, 16, hkv, dim, BF16, table)
+    for s, n in enumerate(lens):
+        cache.fill(s, n, dg)
+    qkv = torch.randn(B, (heads + 2 * hkv) * dim, generator=dg, device="cuda")
+    src = torch.empty_like(qkv)
+    x, y = torch.randn(B, vocab, generator=dg, device="cuda"), torch.empty(B, vocab, device="cuda")
+    temp, nxt = torch.full((B,), 0.5, device="cuda"), i32([-7] * B)
+    r = A.LogitsRules(temperature=temp.data_ptr())
+    rope, pos, n = P.angles(512, dim), i32([m - 1 for m in lens]), i32(lens)
+    q, out, lse = torch.empty(B, heads, dim, device="cuda"), torch.empty(B, heads, dim, device="cuda"), torch.empty(B, heads, device="cuda")
+    ws = torch.empty(L.alb_paged_attn_workspace_bytes(cache.ref(), B, heads), dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        main = torch.cuda.current_stream()
+        src.copy_(qkv)                                    # a copy node
+        side.wait_stream(main)
+        A.check(L.alb_qk_norm_rope_kv_paged(src.data_ptr(), 0, B, heads, None, None, 1e-6, rope.data_ptr(), 512,
+                                            pos.data_ptr(), None, cache.ref(), q.data_ptr(), main.cuda_stream))
+        with torch.cuda.stream(side):
+            A.check(L.alb_logits_process(x.data_ptr(), B, vocab, 0, C.byref(r), y.data_ptr(), 0, nxt.data_ptr(),
+                                         side.cuda_stream))
+        main.wait_stream(side)
+        A.check(L.alb_paged_attn(q.data_ptr(), B, heads, cache.ref(), None, n.data_ptr(), 0, dim ** -0.5,
+                                 ws.data_ptr(), out.data_ptr(), lse.data_ptr(), main.cuda_stream))
+    for _ in range(3):
+        qkv.copy_(torch.randn(qkv.shape, generator=dg, device="cuda"))
+        x.copy_(torch.randn(x.shape, generator=dg, device="cuda"))
+        for t in (src, q, out, lse, y):
+            t.fill_(100.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want, tol = P.rotated(qkv.view(B, -1, dim)[:, :heads], None, rope, torch.tensor(lens) - 1)
+        assert torch.all((q.double().cpu() - want).abs() <= tol)
+        P.check_rows(cache, q, lens, out, lse)
+        assert torch.equal(y, x / temp[:, None]) and torch.equal(nxt, x.argmax(1).int())
