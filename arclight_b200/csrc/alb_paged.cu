@@ -993,11 +993,16 @@ extern "C" int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, 
     ALB_CHECK_ARG(qkv_stride == 0 || (qkv_stride >= dense && qkv_stride % 4 == 0 && qkv_stride < ((int64_t)1 << 31)));
     ALB_CHECK_ARG((((uintptr_t)qkv | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)rope_table | (uintptr_t)q_out) & 15) == 0);
     ALB_CHECK_ARG((((uintptr_t)positions | (uintptr_t)seqs) & 3) == 0);
+    // a token's queries in the place of another's heads would change them before they are read
+    const int64_t stride = qkv_stride ? qkv_stride : dense;
+    const uintptr_t x0 = (uintptr_t)qkv, x1 = x0 + 4 * (uintptr_t)((T - 1) * stride + dense);
+    const uintptr_t y0 = (uintptr_t)q_out, y1 = y0 + 4 * (uintptr_t)(T * n_head * kv->head_dim);
+    ALB_CHECK_ARG((T == 1 && qkv == q_out) || x1 <= y0 || y1 <= x0);
     int * err = device_error_ptr();
     ALB_CUDA_TRY(err ? cudaSuccess : cudaErrorMemoryAllocation);
     auto * f = kv->head_dim == 128 ? (kv->type == ALB_KV_BF16 ? launch_append<128, true> : launch_append<128, false>)
                                    : (kv->type == ALB_KV_BF16 ? launch_append<64, true> : launch_append<64, false>);
-    ALB_CUDA_TRY(f(qkv, qkv_stride ? qkv_stride : dense, T, n_head, q_norm, k_norm, eps, rope_table, max_pos,
+    ALB_CUDA_TRY(f(qkv, stride, T, n_head, q_norm, k_norm, eps, rope_table, max_pos,
                    positions, seqs, v, q_out, err, (cudaStream_t)stream));
     return ALB_OK;
 }

@@ -242,7 +242,7 @@ typedef struct {
  * the table's pages, a sequence >= n_seqs or a page outside [0, n_pages) skips
  * the token and alb_device_error() reports 4.  Two tokens with the same cell
  * leave values of either there.  qkv, q_norm, k_norm, rope_table and q_out are
- * 16-byte aligned. */
+ * 16-byte aligned; q_out does not overlap qkv (for one token it may be qkv). */
 ALB_API int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, int64_t T, int32_t n_head,
                                       const float * q_norm, const float * k_norm, float eps, const float * rope_table,
                                       int32_t max_pos, const int32_t * positions, const int32_t * seqs,

@@ -113,3 +113,19 @@ def test_structures_lie_as_in_the_header(tmp_path):
         want.append(C.sizeof(cls))
         want += [getattr(cls, f).offset for f, _ in cls._fields_]
     assert got == want
+
+
+def test_append_refusals_name_their_reason():
+    """With the queries well away from the input, each refusal is its own, and an overlap is one."""
+    ok, far = cache(), 1 << 30
+    for bad, why in ((dict(qkv=None), b"qkv"), (dict(rope=None), b"rope_table"), (dict(pos=None), b"positions"),
+                     (dict(T=0), b"T > 0"), (dict(T=1 << 30), b"T < "), (dict(heads=0), b"n_head > 0"),
+                     (dict(max_pos=0), b"max_pos > 0"), (dict(eps=-1.0), b"eps"), (dict(qkv=P + 4), b"& 15"),
+                     (dict(kn=P + 2), b"& 15"), (dict(stride=12 * 128 - 4), b"qkv_stride"), (dict(pos=P + 2), b"& 3")):
+        assert append(ok, **{**dict(q=far), **bad}) == A.ALB_ERR_INVALID, bad
+        message = A.lib().alb_last_error()
+        assert why in message and b"q_out ==" not in message and b"qkv == q_out" not in message, (bad, message)
+    row = 12 * 128 * 4
+    for q, T in ((P, 3), (P + row, 2), (P + 2 * row - 16, 2), (P - 16, 1), (P + 16, 1), (P - 3 * 8 * 128 * 4 + 16, 3)):
+        assert append(ok, qkv=P + (1 << 20), q=q + (1 << 20), T=T) == A.ALB_ERR_INVALID, (q, T)
+        assert b"qkv == q_out" in A.lib().alb_last_error()

@@ -316,3 +316,16 @@ def test_captured_calls_on_streams_that_fork_and_join():
         assert torch.all((q.double().cpu() - want).abs() <= tol)
         P.check_rows(cache, q, lens, out, lse)
         assert torch.equal(y, x / temp[:, None]) and torch.equal(nxt, x.argmax(1).int())
+
+
+# --------------------------------------------------------------------------------------------------- in place
+def test_one_token_appended_in_place():
+    heads, hkv, dim = 8, 2, 128
+    dg = torch.Generator(device="cuda").manual_seed(3)
+    cache = P.Cache(4, 16, hkv, dim, F16, torch.arange(2)[None])
+    x = torch.randn(1, (heads + 2 * hkv) * dim, generator=dg, device="cuda")
+    w, rope, pos = 1 + 0.1 * torch.randn(dim, generator=dg, device="cuda"), P.angles(32, dim), i32([17])
+    want = P.append(cache, x, heads, w, w, rope, pos)
+    kept = x.clone()
+    P.append(cache, x, heads, w, w, rope, pos, q=x)
+    assert torch.equal(x[:, :heads * dim], want.view(1, -1)) and torch.equal(x[:, heads * dim:], kept[:, heads * dim:])
