@@ -1023,6 +1023,9 @@ extern "C" int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, c
     ALB_CHECK_ARG(scale > 0.0f && std::isfinite(scale));
     ALB_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0);
     ALB_CHECK_ARG((((uintptr_t)lengths | (uintptr_t)seqs | (uintptr_t)lse) & 3) == 0);
+    // in place is fine: a unit reads its queries before it writes, and nothing else reads them
+    const uintptr_t x0 = (uintptr_t)q, y0 = (uintptr_t)out, bytes = 4 * (uintptr_t)(n_rows * n_head * kv->head_dim);
+    ALB_CHECK_ARG(x0 == y0 || x0 + bytes <= y0 || y0 + bytes <= x0);
     PaArgs a = {};
     a.q = q; a.kv = v; a.seqs = seqs; a.lengths = lengths; a.n_rows = n_rows; a.Hq = n_head; a.G = n_head / v.Hkv;
     a.window = window; a.scale_log2 = scale * 1.44269504f; a.out = out; a.lse = lse;

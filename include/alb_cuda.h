@@ -271,7 +271,8 @@ ALB_API int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, int
  * new lengths, tables and queries in the same buffers.  workspace:
  * alb_paged_attn_workspace_bytes() bytes (up to 9 MB, whatever the batch), 16-byte
  * aligned, no state kept in it between calls; calls that may overlap in time (other streams, two captured
- * graphs replayed side by side) need one each.  q and out are 16-byte aligned. */
+ * graphs replayed side by side) need one each.  q and out are 16-byte aligned; out may be q itself, but not overlap it
+ * otherwise. */
 ALB_API size_t alb_paged_attn_workspace_bytes(const alb_paged_kv * kv, int64_t n_rows, int32_t n_head);
 ALB_API int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, const alb_paged_kv * kv,
                            const int32_t * seqs, const int32_t * lengths, int32_t window, float scale,

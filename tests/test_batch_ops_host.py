@@ -129,3 +129,10 @@ def test_append_refusals_name_their_reason():
     for q, T in ((P, 3), (P + row, 2), (P + 2 * row - 16, 2), (P - 16, 1), (P + 16, 1), (P - 3 * 8 * 128 * 4 + 16, 3)):
         assert append(ok, qkv=P + (1 << 20), q=q + (1 << 20), T=T) == A.ALB_ERR_INVALID, (q, T)
         assert b"qkv == q_out" in A.lib().alb_last_error()
+
+
+def test_attention_queries_and_outputs_do_not_half_overlap():
+    ok, at, size = cache(), 1 << 20, 3 * 8 * 128 * 4
+    for out in (at + 16, at - 16, at + size - 16, at - size + 16, at + 128 * 4):
+        assert attend(ok, q=at, out=out) == A.ALB_ERR_INVALID, out
+        assert b"y0" in A.lib().alb_last_error()

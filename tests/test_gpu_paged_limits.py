@@ -319,6 +319,26 @@ def test_captured_calls_on_streams_that_fork_and_join():
 
 
 # --------------------------------------------------------------------------------------------------- in place
+@pytest.mark.parametrize("heads,hkv,dim,typ", [(8, 2, 128, F16), (14, 2, 64, BF16), (17, 1, 128, BF16)])
+def test_outputs_in_the_place_of_the_queries(heads, hkv, dim, typ):
+    """Whole units, units cut into pieces, empty rows and padding."""
+    lens = [30000, 0, 5, 300, -1, 1]
+    gen = torch.Generator().manual_seed(dim)
+    dg = torch.Generator(device="cuda").manual_seed(heads)
+    table, pool = P.make_table([max(n, 0) for n in lens], 16, gen)
+    cache = P.Cache(pool, 16, hkv, dim, typ, table)
+    for s, n in enumerate(lens):
+        if n > 0:
+            cache.fill(s, n, dg)
+    q = torch.randn(len(lens), heads, dim, generator=dg, device="cuda")
+    want, lse = P.attend(cache, q, i32(lens))
+    want[4] = q[4]                                        # padding keeps what is there
+    for _ in range(5):
+        both = q.clone()
+        _, l2 = P.attend(cache, both, i32(lens), out=both)
+        assert torch.equal(both, want) and torch.equal(l2, lse)
+
+
 def test_one_token_appended_in_place():
     heads, hkv, dim = 8, 2, 128
     dg = torch.Generator(device="cuda").manual_seed(3)
