@@ -13,10 +13,12 @@
 // mask, maximum.  The CTAs' maxima go to CTA 0's shared memory.
 //
 // Bound by instruction issue and the chain of dependent steps, not by HBM: 256
-// rows of 151936 with histories to 4096 and masks take 83 us (314 MB, 3.8 TB/s;
-// about 60 issued instructions per group of four tokens and 80 per id and CTA that
-// reads it), 48 rows with biases and masks 20 us, 64 rows of 32003 with histories
-// to 8192 13 us, one row 4.8 us.  Other shapes that were measured on the first of
+// rows of 151936 with histories to 4096 and masks take 83 us (314 MB, 3.8 TB/s).
+// A warp issues about 1700 instructions there: 520 for copy and maximum of its nine
+// groups of four tokens a lane, 190 for the temperature, 240 for the mask, 330 to
+// look into the table, and 110 for each id that its lanes read, four on average.
+// 48 rows with biases and masks take 20 us, 64 rows of 32003 with histories to 8192
+// 13 us, one row 4.8 us.  Other shapes that were measured on the first of
 // these: ids counted across the cluster in distributed shared memory 113 us
 // (frequent ids queue up at their owner), the share brought to shared memory by
 // bulk copies 124 us (room for two CTAs), slots by a bit map's running count 97 us

@@ -196,22 +196,27 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // window say so), and no sum passes the largest |V|; q is scaled below 2^-9, so
 // that 128 products with any K fit too.
 //
-// Bound by HBM: 48 sequences of 8k to 32k cells (32 / 8 heads of 128) stream 4.2 GB
-// in 622 us, 6.75 TB/s; 37 ragged ones 110 us (bf16, its three parts in one
-// product for up to four heads).  bf16 with five to eight heads a group takes two
-// products and keeps the third parts of q in shared memory: 64 sequences of 4k to
-// 8k cells 5.3 TB/s (4.3 with all parts in registers, which spill), where four
-// heads stream 6.6.  Units of 16 heads take one product a part of all 16: 200
-// sequences of 4k to 8k cells with 16 / 1 heads 136 us in fp16, 4.6 TB/s, and 153
-// in bf16 (two units of eight, which read K and V twice: 183 and 226).  A warp has a tile of K and V
-// (8 KB) in flight while it works on the one before, twelve warps an SM 96 KB; 16
-// warps at 128 registers spill (907 us), eight at 255 hold too little (676 us).  K
-// through the L1 cache, whose half lines the next load takes, is worth a tenth on
-// short calls.  Few rows are bound by the chain of dependent loads (lengths, page,
-// K and V; the join: what is unfinished, its pieces): one sequence of 640 cells
-// 8.3 us, of 32768 cells 32 us, 200 windows of single cells 22 us.  A unit's setup
-// weighs six tiles (0: 29 us for the windows and 122 for the ragged batch, 12:
-// 22.8 and 110).
+// Bound by HBM: 48 sequences of 8k to 32k cells (32 / 8 heads of 128) stream 6.6 to
+// 6.75 TB/s, 4.2 GB in 622 us (lengths drawn anew hold 3.8 to 4.4 GB: 575 to 664
+// us); 37 ragged ones take 109 us (bf16, its three parts in one product for up to
+// four heads).  bf16 with five to eight heads a group takes two products and keeps
+// the third parts of q in shared memory: 64 sequences of 4k to 8k cells 303 us, 5.3
+// TB/s (4.3 with all parts in registers), where four heads stream 6.6.  Units of 16
+// heads take one product a part of all 16: 200 sequences of 4k to 8k cells with
+// 16 / 1 heads 136 us in fp16, 4.6 TB/s, and 154 in bf16 (two units of eight, which
+// read K and V twice: 183 and 226).
+//
+// A warp has a tile of K and V (8 KB) in flight while it works on the one before,
+// twelve warps an SM 96 KB; 16 warps at 128 registers spill (907 us for the 48
+// sequences), eight at 255 hold too little (676 us), which is what units of 16 run
+// with: 64 KB an SM in flight for two thirds of the rate.  At D = 128 all kinds
+// spill a little: 36 bytes a thread for bf16 with up to four heads, 44 for fp16, 80
+// for bf16 of 16 heads and 128 of five to eight (at D = 64 none).  K through the L1 cache, whose half lines the next load takes, is worth
+// a tenth on short calls.  Few rows are bound by the chain of dependent loads
+// (lengths, page, K and V; the join: what is unfinished, its pieces): one sequence
+// of 640 cells 8.2 us (bf16 8.4), of 32768 cells 32 us, 200 windows of single cells
+// 22 us.  A unit's setup weighs six tiles (0: 29 us for the windows and 122 for the
+// ragged batch, 12: 22.8 and 110).
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = 32 * PA_WARPS;
 // CTAs per SM: what the registers allow (168 a thread for units of 8 heads, 255 for units of 16)
@@ -564,8 +569,8 @@ k_paged_attn(const __grid_constant__ PaArgs a) {
 #pragma unroll
             for (int b = 0; b < SUB; ++b) {
                 // Each product truncates its sums, so the small parts are summed apart from the first (in rows
-                // 8-15 for R = 1, in sums of their own for R = 2), and chains are short: the worst of 6000 random
-                // cases is 6e-7 off, with one chain a row 1.8e-6.
+                // 8-15 for R = 1, in sums of their own for R = 2), and chains are short: of 6000 random batches the
+                // worst has outputs 6e-7 off (norm of the errors by norm of the outputs), with one chain a row 1.8e-6.
                 float s[2][2][4], small[2][4];   // (two chains each, halves of the k steps)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
