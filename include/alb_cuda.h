@@ -264,17 +264,16 @@ ALB_API int alb_qk_norm_rope_kv_paged(const float * qkv, int64_t qkv_stride, int
  * their type, scores and scale * |q| below 1e34: an infinity or NaN in K or V makes
  * the rows' heads that meet it infinite or NaN, one in a query that head alone.
  * (bf16 results are held to 1e-44 times the positions of table or window besides:
- * 1e-39 for 100 000 of them.)  A sequence outside
- * [0, n_seqs) leaves its row without cells, a length beyond the table is cut to it,
- * and the cells of a page outside [0, n_pages) are not seen; each makes
- * alb_device_error() report 4.  A prompt's tokens may be rows too (their own
- * lengths), each reading its cells anew.
+ * 1e-39 for 100 000 of them.)  A sequence outside [0, n_seqs) leaves its row without
+ * cells, a length beyond the table is cut to it, and the cells of a page outside
+ * [0, n_pages) are not seen; each makes alb_device_error() report 4.  A prompt's
+ * tokens may be rows too (their own lengths), each reading its cells anew.
  * Nothing depends on the lengths but the work, so a captured call replays with
  * new lengths, tables and queries in the same buffers.  workspace:
  * alb_paged_attn_workspace_bytes() bytes (up to 9 MB, whatever the batch), 16-byte
  * aligned, no state kept in it between calls; calls that may overlap in time (other
- * streams, two captured graphs replayed side by side) need one each.  q and out are 16-byte aligned; out may be q itself, but not overlap it
- * otherwise. */
+ * streams, two captured graphs replayed side by side) need one each.  q and out are
+ * 16-byte aligned; out may be q itself, but not overlap it otherwise. */
 ALB_API size_t alb_paged_attn_workspace_bytes(const alb_paged_kv * kv, int64_t n_rows, int32_t n_head);
 ALB_API int alb_paged_attn(const float * q, int64_t n_rows, int32_t n_head, const alb_paged_kv * kv,
                            const int32_t * seqs, const int32_t * lengths, int32_t window, float scale,
