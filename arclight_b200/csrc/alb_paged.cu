@@ -198,7 +198,7 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 //
 // Bound by HBM: 48 sequences of 8k to 32k cells (32 / 8 heads of 128) stream 6.6 to
 // 6.75 TB/s, 4.2 GB in 622 us (lengths drawn anew hold 3.8 to 4.4 GB: 575 to 664
-// us); 37 ragged ones take 109 us (bf16, its three parts in one product for up to
+// us and more); 37 ragged ones take 109 us (bf16, its three parts in one product for up to
 // four heads).  bf16 with five to eight heads a group takes two products and keeps
 // the third parts of q in shared memory: 64 sequences of 4k to 8k cells 303 us, 5.3
 // TB/s (4.3 with all parts in registers), where four heads stream 6.6.  Units of 16
@@ -211,12 +211,12 @@ k_qk_norm_rope_kv_paged(const float * __restrict__ qkv, int64_t qkv_stride, int 
 // sequences), eight at 255 hold too little (676 us), which is what units of 16 run
 // with: 64 KB an SM in flight for two thirds of the rate.  At D = 128 all kinds
 // spill a little: 36 bytes a thread for bf16 with up to four heads, 44 for fp16, 80
-// for bf16 of 16 heads and 128 of five to eight (at D = 64 none).  K through the L1 cache, whose half lines the next load takes, is worth
-// a tenth on short calls.  Few rows are bound by the chain of dependent loads
-// (lengths, page, K and V; the join: what is unfinished, its pieces): one sequence
-// of 640 cells 8.2 us (bf16 8.4), of 32768 cells 32 us, 200 windows of single cells
-// 22 us.  A unit's setup weighs six tiles (0: 29 us for the windows and 122 for the
-// ragged batch, 12: 22.8 and 110).
+// for bf16 of 16 heads and 128 of five to eight (at D = 64 none).  K through the L1
+// cache, whose half lines the next load takes, is worth a tenth on short calls.  Few
+// rows are bound by the chain of dependent loads (lengths, page, K and V; the join:
+// what is unfinished, its pieces): one sequence of 640 cells 8.2 us (bf16 8.4), of
+// 32768 cells 32 us, 200 windows of single cells 22 us.  A unit's setup weighs six
+// tiles (0: 29 us for the windows and 122 for the ragged batch, 12: 22.8 and 110).
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = 32 * PA_WARPS;
 // CTAs per SM: what the registers allow (168 a thread for units of 8 heads, 255 for units of 16)

@@ -317,8 +317,8 @@ typedef struct {
  * when nothing but -INFINITY and NaN is left.  Negative ids in history and
  * bias_ids are skipped; ids >= n_vocab, lengths beyond history_stride (cut to
  * it), bias offsets outside [0, n_bias] (cut) or falling (no entries) and mask rows
- * >= n_allow (no mask) make alb_device_error() report 4.  Extends sample_none (sampler.cpp:34-36),
- * the reference's only sampler.  n_vocab <= 450000, rows < 2^24. */
+ * >= n_allow (no mask) make alb_device_error() report 4.  Extends sample_none
+ * (sampler.cpp:34-36), the reference's only sampler.  n_vocab <= 450000, rows < 2^24. */
 ALB_API int alb_logits_process(const float * logits, int64_t rows, int64_t n_vocab, int64_t stride,
                                const alb_logits_rules * rules, float * out, int64_t out_stride, int32_t * next_token,
                                void * stream);
